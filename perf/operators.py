@@ -1,0 +1,459 @@
+"""Cases of the feed-forward operators: layer norm, the product with bias, activation and residual in its
+epilogue, and the AdamW step over many tensors. With ``own`` false, run() computes them in elementary torch
+operations in 32 bits; with ``own`` true, it makes the calls a program makes of sehip.
+
+The definitions (R rows, C features; x [M, K], W [N, K]):
+
+  layer norm   h = (x - mean) / sqrt(var + eps), y = h w + b, and the gradients of x, w, b
+  product      y = act(x W^T + b) + residual, and the gradients of x, W, b, residual
+  AdamW        m' = m + (1 - b1)(g - m), v' = b2 v + (1 - b2) g^2,
+               p' = p (1 - lr wd) - lr / (1 - b1^t) m' / (sqrt(v') / sqrt(1 - b2^t) + eps)
+               32: m and v in fp32. 8: m and sqrt(v) as e4m3 values times one power of two for each 128 elements,
+               rounded stochastically with a counter hash of (seed, step, tensor, element)."""
+import math
+import os
+import sys
+
+import torch
+
+own = False
+
+BLOCK = 128                     # elements that share a power of two
+LR, BETAS, EPS, DECAY = 1e-3, (0.9, 0.999), 1e-8, 1e-2
+LN_EPS = 1e-5
+TYPES = {"f32": torch.float32, "bf16": torch.bfloat16, "f16": torch.float16}
+SIZE = {"f32": 4, "bf16": 2, "f16": 2}
+ACTS = ("none", "relu", "gelu", "gelu_tanh", "silu")
+
+
+def _sehip():
+    """The package's folder is put on the path as bench.py does it."""
+    at = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "speech-enhancement_amd")
+    if at not in sys.path:
+        sys.path.insert(0, at)
+    from sehip import linear, norm, optim
+    return linear, norm, optim
+
+
+# ---------------------------------------------------------------------------------------------- the cases
+
+
+def _norm(name, dtype, rows, width, train):
+    return {"name": name, "op": "norm", "dtype": dtype, "rows": rows, "width": width, "train": train}
+
+
+def _linear(name, dtype, rows, inputs, outputs, act, residual, train):
+    return {"name": name, "op": "linear", "dtype": dtype, "rows": rows, "inputs": inputs, "outputs": outputs,
+            "act": act, "residual": residual, "train": train}
+
+
+def _adamw(name, dtype, bits, blocks, width, hidden):
+    return {"name": name, "op": "adamw", "dtype": dtype, "bits": bits, "blocks": blocks, "width": width,
+            "hidden": hidden}
+
+
+def listed():
+    return [
+        # one frame of a stream through a 1024-wide layer
+        _norm("norm one frame", "bf16", 1, 1024, False),
+        # a training batch of 64 utterances of 4 s (403 frames each) at the 514 rows of a spectrum: an odd width
+        _norm("norm batch odd f32", "f32", 25792, 514, True),
+        # a wide model's training batch
+        _norm("norm wide bf16", "bf16", 32768, 4096, True),
+        # the first product of a feed-forward block for one frame of a stream
+        _linear("linear one frame", "bf16", 1, 1024, 4096, "gelu", False, False),
+        # the second product for sixteen streams served together
+        _linear("linear few rows f16", "f16", 16, 4096, 1024, "none", True, False),
+        # the two products of a 512-wide block on the training batch above
+        _linear("linear up bf16", "bf16", 25792, 512, 2048, "gelu", False, True),
+        _linear("linear down bf16", "bf16", 25792, 2048, 512, "none", True, True),
+        # 30 s at 48 kHz (9002 frames) in fp32, spectrum rows in and out
+        _linear("linear odd f32", "f32", 9002, 514, 1030, "silu", True, True),
+        # a wide model's first product in training
+        _linear("linear large bf16", "bf16", 16384, 4096, 8192, "gelu_tanh", False, True),
+        # every tensor of a small model: many short ones, where launches and the host count
+        _adamw("adamw 8 small", "f32", 8, 4, 96, 388),
+        # 16-bit parameters whose states stay in 32 bits
+        _adamw("adamw 32 bf16", "bf16", 32, 8, 1024, 4096),
+        # a large fp32 model with its states in 8 bits
+        _adamw("adamw 8 large", "f32", 8, 10, 2048, 8192),
+    ]
+
+
+def _log(rng, lo, hi):
+    return int(round(math.exp(rng.uniform(math.log(lo), math.log(hi)))))
+
+
+def draw(rng):
+    op = rng.choice(("norm", "norm", "linear", "linear", "linear", "adamw"))
+    dtype = rng.choice(("f32", "bf16", "bf16", "f16"))
+    if op == "norm":
+        width = _log(rng, 16, 8192)
+        rows = _log(rng, 1, min(65536, 32768 * 4096 * 2 // (width * SIZE[dtype])))
+        c = _norm("", dtype, rows, width, rng.random() < 0.7)
+    elif op == "linear":
+        few = rng.random() < 0.3
+        inputs, outputs = _log(rng, 64, 4096), _log(rng, 64, 8192)
+        if rng.random() < 0.5:
+            inputs, outputs = 64 * max(1, inputs // 64), 64 * max(1, outputs // 64)
+        rows = _log(rng, 1, 32) if few else _log(rng, 33, 16384)
+        if dtype == "f32":       # three terms a product
+            rows = min(rows, 8192)
+        # relu's slope jumps at zero, where two sums of 32 bits may fall on either side: 16 bits only
+        acts = [a for a in ACTS if a != "relu" or dtype != "f32"]
+        c = _linear("", dtype, rows, inputs, outputs, rng.choice(acts), rng.random() < 0.5, not few)
+    else:
+        width, hidden = _log(rng, 32, 1536), _log(rng, 64, 4096)
+        c = _adamw("", dtype, rng.choice((8, 8, 32)), rng.randint(1, 8), width, hidden)
+    del c["name"]
+    return c
+
+
+def _shapes(case):
+    """The parameters of `blocks` pre-norm feed-forward blocks: norm, product up, product down."""
+    w, h = case["width"], case["hidden"]
+    return [(w,), (w,), (h, w), (h,), (w, h), (w,)] * case["blocks"]
+
+
+def work(case):
+    e = SIZE[case["dtype"]]
+    if case["op"] == "norm":
+        n = case["rows"] * case["width"]
+        # forward: x in, y out; training: x and dy in, y and dx out (and the vectors)
+        return {"bytes": (4 if case["train"] else 2) * n * e + (4 if case["train"] else 2) * case["width"] * e,
+                "flops": (20 if case["train"] else 8) * n}
+    if case["op"] == "linear":
+        m, k, n, r = case["rows"], case["inputs"], case["outputs"], int(case["residual"])
+        b = m * k + n * k + n + (1 + r) * m * n
+        if case["train"]:
+            b += m * n + m * k + n * k + n
+        return {"bytes": b * e, "flops": (6 if case["train"] else 2) * m * n * k}
+    total = sum(math.prod(s) for s in _shapes(case))
+    states = 16 if case["bits"] == 32 else 4 + 4 / BLOCK
+    return {"bytes": total * (3 * e + states), "flops": 16 * total}
+
+
+# ---------------------------------------------------------------------------------------------- the inputs
+
+
+def prepare(case, seed):
+    dev = torch.device("cuda")
+    g = torch.Generator(device=dev).manual_seed(seed)
+    dt = TYPES[case["dtype"]]
+
+    def normal(*shape):
+        return torch.randn(*shape, generator=g, device=dev)
+
+    if case["op"] == "norm":
+        # frames of different loudness, features with a mean of their own
+        r, c = case["rows"], case["width"]
+        x = (normal(r, c) + 0.5 * normal(c)) * torch.exp(0.7 * normal(r, 1))
+        m = torch.nn.LayerNorm(c, eps=LN_EPS, device=dev, dtype=dt)
+        with torch.no_grad():
+            m.weight.copy_(1 + 0.2 * normal(c))
+            m.bias.copy_(0.1 * normal(c))
+        x = x.to(dt).requires_grad_(case["train"])
+        return {"case": case, "x": x, "module": m, "dy": normal(r, c).to(dt) if case["train"] else None}
+    if case["op"] == "linear":
+        r, k, n = case["rows"], case["inputs"], case["outputs"]
+        m = torch.nn.Linear(k, n, device="meta", dtype=dt).to_empty(device=dev)
+        with torch.no_grad():
+            m.weight.copy_(normal(n, k) / math.sqrt(k))
+            m.bias.copy_(0.1 * normal(n))
+        acts = {"none": torch.nn.Identity(), "relu": torch.nn.ReLU(), "gelu": torch.nn.GELU(),
+                "gelu_tanh": torch.nn.GELU("tanh"), "silu": torch.nn.SiLU()}
+        x = normal(r, k).to(dt).requires_grad_(case["train"])
+        res = normal(r, n).to(dt).requires_grad_(case["train"]) if case["residual"] else None
+        return {"case": case, "x": x, "module": m, "act": acts[case["act"]], "residual": res,
+                "dy": (0.1 * normal(r, n)).to(dt) if case["train"] else None}
+    # one buffer for each kind, every tensor at a block of its own (a program's tensors lie apart, each aligned)
+    shapes = _shapes(case)
+    sizes = [math.prod(t) for t in shapes]
+    at = [0]
+    for n in sizes:
+        at.append(at[-1] + -(-n // BLOCK) * BLOCK)
+    spots = list(zip(shapes, sizes, at))
+    s = {"case": case, "step": 200 + seed % 1000, "seed": seed % 65536, "flat": {}}
+
+    def keep(kind, dtype, unit, tensors):
+        s["flat"][kind] = torch.zeros(at[-1] // unit, device=dev, dtype=torch.uint8 if dtype.itemsize == 1 else dtype).view(dtype)
+        s[kind] = [s["flat"][kind][o // unit:o // unit + -(-n // unit)].view(t if unit == 1 else -1) for t, n, o in spots]
+        for to, new in zip(s[kind], tensors):
+            _store(to, new)
+
+    keep("p", dt, 1, (0.05 * normal(*t) for t in shapes))
+    keep("g", dt, 1, (0.01 * normal(*t) * torch.exp(normal(*t[:1], *[1] * (len(t) - 1))) for t in shapes))
+    m = (0.1 * g.float() + 0.002 * normal(*g.shape) for g in s["g"])
+    q = (0.01 * torch.exp(0.7 * normal(*t)) for t in shapes)
+    if case["bits"] == 32:
+        keep("m", torch.float32, 1, m)
+        keep("v", torch.float32, 1, (t.square() for t in q))
+    else:
+        for a, b, tensors in (("m", "mk", m), ("q", "qk", q)):
+            pairs = [_pack(t, None) for t in tensors]
+            keep(a, torch.float8_e4m3fn, 1, (x for x, _ in pairs))
+            keep(b, torch.float8_e8m0fnu, BLOCK, (x for _, x in pairs))
+    del s["flat"]["g"]
+    return s
+
+
+def _store(to, new):
+    if to.dtype.itemsize == 1:
+        to, new = to.view(torch.uint8), new.view(torch.uint8)
+    to.copy_(new)
+
+
+# ------------------------------------------------------------------------- 8-bit states in elementary operations
+
+
+def _mix(x):
+    """The hash of a counter, on int64 tensors or Python ints that hold 32 bits."""
+    x = (x ^ (x >> 15)) * 0x6A09E667 & 0xFFFFFFFF
+    x = (x ^ (x >> 13)) * 0xBB67AE85 & 0xFFFFFFFF
+    return x ^ (x >> 16)
+
+
+def _key(seed, step, tensor):
+    return _mix(_mix(_mix(seed & 0xFFFFFFFF) + step & 0xFFFFFFFF) + tensor & 0xFFFFFFFF)
+
+
+def _random16(n, key, device):
+    i = torch.arange(n, device=device)
+    h = _mix((i * 0x9E3779B1 + (i >> 32) * 0x243F6A89 + key) & 0xFFFFFFFF)
+    return h & 0xFFFF, h >> 16
+
+
+def _pack(x, h, floor=False):
+    """(e4m3 values, powers of two) of x; h: 16 random bits an element, or None to round to the nearest.
+    floor: a value above zero does not become zero. In 64 bits: a value next to a border."""
+    n = x.numel()
+    pad = -n % BLOCK
+    y = torch.nn.functional.pad(x.reshape(-1).double(), (0, pad)).view(-1, BLOCK)
+    top = y.abs().amax(1, keepdim=True)
+    k = torch.ceil(torch.log2(top / 448)).clamp(-126, 127)
+    k = torch.where(top > 448 * torch.exp2(k), k + 1, torch.where(top <= 448 * torch.exp2(k - 1), k - 1, k))
+    k = k.clamp(-126, 127)
+    a = (y.abs() * torch.exp2(-k)).view(-1)[:n]
+    unit = torch.exp2((torch.frexp(a)[1] - 1).clamp(min=-6).double() - 3)
+    u = 0.5 if h is None else (h.double() + 0.5) / 65536
+    a = torch.floor(a / unit + u) * unit
+    if floor:
+        a = torch.where(x.reshape(-1) > 0, a.clamp(min=2.0 ** -9), a)
+    a = torch.copysign(a, x.reshape(-1).double())
+    code = (k.view(-1) + 127).to(torch.uint8).view(torch.float8_e8m0fnu)
+    return a.float().to(torch.float8_e4m3fn).view(x.shape), code
+
+
+def _unpack(a, code):
+    n = a.numel()
+    k = torch.exp2(code.view(torch.uint8).float() - 127)
+    return (a.reshape(-1).float() * k.repeat_interleave(BLOCK)[:n]).view(a.shape)
+
+
+# ---------------------------------------------------------------------------------------------- one pass
+
+
+def run(state):
+    op = state["case"]["op"]
+    if own:
+        return {"norm": _own_norm, "linear": _own_linear, "adamw": _own_adamw}[op](state)
+    with torch.no_grad():
+        return {"norm": _plain_norm, "linear": _plain_linear, "adamw": _plain_adamw}[op](state)
+
+
+def _plain_norm(s):
+    x, w, b, dt = s["x"].float(), s["module"].weight.float(), s["module"].bias.float(), s["x"].dtype
+    d = x - x.mean(1, keepdim=True)
+    rstd = 1 / torch.sqrt((d * d).mean(1, keepdim=True) + LN_EPS)
+    h = d * rstd
+    y = (h * w + b).to(dt)
+    if s["dy"] is None:
+        return y
+    dy = s["dy"].float()
+    a = dy * w
+    dx = rstd * (a - a.mean(1, keepdim=True) - h * (a * h).mean(1, keepdim=True))
+    return y, dx.to(dt), (dy * h).sum(0).to(dt), dy.sum(0).to(dt)
+
+
+def _own_norm(s):
+    _, norm, _ = _sehip()
+    m = s["module"]
+    if s["dy"] is None:
+        with torch.no_grad():
+            return norm.layer_norm(m, s["x"])
+    y = norm.layer_norm(m, s["x"])
+    return (y.detach(), *torch.autograd.grad(y, (s["x"], m.weight, m.bias), s["dy"]))
+
+
+def _act(name, z):
+    """act(z) and act'(z)."""
+    if name == "none":
+        return z, torch.ones_like(z)
+    if name == "relu":
+        return z * (z > 0), (z > 0).to(z.dtype)
+    if name == "silu":
+        p = 1 / (1 + torch.exp(-z))
+        return z * p, p * (1 + z * (1 - p))
+    if name == "gelu":
+        p = 0.5 * (1 + torch.erf(z * math.sqrt(0.5)))
+        return z * p, p + z * torch.exp(-0.5 * z * z) / math.sqrt(2 * math.pi)
+    c = math.sqrt(2 / math.pi)
+    t = torch.tanh(c * (z + 0.044715 * z * z * z))
+    return 0.5 * z * (1 + t), 0.5 * (1 + t) + 0.5 * z * (1 - t * t) * c * (1 + 3 * 0.044715 * z * z)
+
+
+def _plain_linear(s):
+    x, w, b, dt = s["x"].float(), s["module"].weight.float(), s["module"].bias.float(), s["x"].dtype
+    z = x @ w.t() + b
+    y, slope = _act(s["case"]["act"], z)
+    if s["residual"] is not None:
+        y = y + s["residual"].float()
+    y = y.to(dt)
+    if s["dy"] is None:
+        return y
+    g = s["dy"].float() * slope
+    out = (y, (g @ w).to(dt), (g.t() @ x).to(dt), g.sum(0).to(dt))
+    return out if s["residual"] is None else (*out, s["dy"])
+
+
+def _own_linear(s):
+    linear, _, _ = _sehip()
+    m = s["module"]
+    if s["dy"] is None:
+        with torch.no_grad():
+            return linear.linear_act(s["x"], m, s["act"], s["residual"])
+    y = linear.linear_act(s["x"], m, s["act"], s["residual"])
+    of = (s["x"], m.weight, m.bias) + (() if s["residual"] is None else (s["residual"],))
+    return (y.detach(), *torch.autograd.grad(y, of, s["dy"]))
+
+
+def _plain_step(p, g, m, v, step):
+    """The step of one tensor in 32 bits: the new m and v; p is written."""
+    b1, b2 = BETAS
+    g = g.float()
+    m = m + (1 - b1) * (g - m)
+    v = b2 * v + (1 - b2) * g * g
+    new = p.float() * (1 - LR * DECAY) - (LR / (1 - b1 ** step)) * m / (
+        torch.sqrt(v) / math.sqrt(1 - b2 ** step) + EPS)
+    p.copy_(new)
+    return m, v
+
+
+def _plain_one8(s, i):
+    m, v = _plain_step(s["p"][i], s["g"][i], _unpack(s["m"][i], s["mk"][i]), _unpack(s["q"][i], s["qk"][i]).square(),
+                       s["step"])
+    lo, hi = _random16(m.numel(), _key(s["seed"], s["step"], i), m.device)
+    for a, k, new in (("m", "mk", _pack(m, lo)), ("q", "qk", _pack(torch.sqrt(v), hi, True))):
+        _store(s[a][i], new[0])
+        _store(s[k][i], new[1])
+
+
+def _plain_one32(s, i):
+    m, v = _plain_step(s["p"][i], s["g"][i], s["m"][i], s["v"][i], s["step"])
+    s["m"][i].copy_(m)
+    s["v"][i].copy_(v)
+
+
+def _plain_adamw(s):
+    one = _plain_one8 if s["case"]["bits"] == 8 else _plain_one32
+    [one(s, i) for i in range(len(s["p"]))]
+    return s["flat"]
+
+
+def _own_adamw(s):
+    _, _, optim = _sehip()
+    kw = dict(step=s["step"], lr=LR, betas=BETAS, eps=EPS, weight_decay=DECAY)
+    if s["case"]["bits"] == 8:
+        optim.adamw8_(s["p"], s["g"], s["m"], s["mk"], s["q"], s["qk"], seed=s["seed"], **kw)
+    else:
+        optim.adamw32_(s["p"], s["g"], s["m"], s["v"], **kw)
+    return s["flat"]
+
+
+# ---------------------------------------------------------------------------------------------- in 64 bits
+
+
+def exact(case, seed):
+    """The definitions in 64 bits; the gradients of norm and product by automatic differentiation."""
+    s = prepare(case, seed)
+    if case["op"] == "adamw":
+        return _exact_adamw(s)
+
+    def leaf(t):
+        return None if t is None else t.detach().double().requires_grad_(True)
+
+    x, w, b = leaf(s["x"]), leaf(s["module"].weight), leaf(s["module"].bias)
+    if case["op"] == "norm":
+        mu = x.sum(1, keepdim=True) / x.shape[1]
+        y = w * ((x - mu) * torch.rsqrt(((x - mu) ** 2).sum(1, keepdim=True) / x.shape[1] + LN_EPS)) + b
+        of = (x, w, b)
+    else:
+        r = leaf(s["residual"])
+        z = torch.addmm(b, x, w.t())
+        y = {"none": lambda: z * 1, "relu": lambda: z.clamp(min=0), "silu": lambda: z * torch.sigmoid(z),
+             "gelu": lambda: z * (1 - 0.5 * torch.erfc(z / 2 ** 0.5)),
+             "gelu_tanh": lambda: z * torch.sigmoid(2 * (2 / math.pi) ** 0.5 * (z + 0.044715 * z ** 3))}[case["act"]]()
+        if r is not None:
+            y = y + r
+        of = (x, w, b) if r is None else (x, w, b, r)
+    if s["dy"] is None:
+        return y.detach()
+    return (y.detach(), *torch.autograd.grad(y, of, s["dy"].double()))
+
+
+def _e4m3():
+    """Every magnitude of the format, in order: sixteen binades of eight, the last value left out."""
+    v = [(f / 8) * 2.0 ** -6 if e == 0 else (1 + f / 8) * 2.0 ** (e - 7) for e in range(16) for f in range(8)]
+    return torch.tensor(v[:-1], dtype=torch.float64)
+
+
+def _exact_pack(x, h, floor):
+    grid = _e4m3().to(x.device)
+    a, n = x.abs().reshape(-1), x.numel()
+    tops = a[:n - n % BLOCK].view(-1, BLOCK).amax(1) if n >= BLOCK else a.new_zeros(0)
+    if n % BLOCK:
+        tops = torch.cat([tops, a[n - n % BLOCK:].max()[None]])
+    f, e = torch.frexp(tops)              # tops = f 2^e with f in [1/2, 1): 448 = 7/8 2^9
+    k = torch.where(f <= 0.875, e - 9, e - 8)
+    k = torch.where(tops > 0, k, torch.full_like(k, -126)).clamp(-126, 127)
+    a = torch.ldexp(a, -k.repeat_interleave(BLOCK)[:n])
+    at = (torch.searchsorted(grid, a, right=True) - 1)
+    lo, hi = grid[at], grid[(at + 1).clamp(max=len(grid) - 1)]
+    up = (a - lo) / (hi - lo).clamp(min=1e-30) + (h.double() + 0.5) / 65536 >= 1
+    a = torch.where(up, hi, lo)
+    if floor:
+        a = torch.where((a == 0) & (x.reshape(-1) > 0), grid[1], a)
+    return (torch.sign(x.reshape(-1)) * a).view(x.shape), torch.ldexp(torch.ones_like(tops), k)
+
+
+def _exact_adamw(s):
+    b1, b2 = BETAS
+    t = s["step"]
+    got = {k: torch.zeros(x.numel(), device=x.device, dtype=torch.float64) for k, x in s["flat"].items()}
+    for k in ("mk", "qk"):
+        if k in got:
+            got[k] += s["flat"][k].view(torch.uint8).double().sub(127).exp2()
+    at = 0
+    for i, g in enumerate(s["g"]):
+        n = g.numel()
+        blocks = -(-n // BLOCK)
+        here = slice(at, at + n)
+        g, p = g.double().view(-1), s["p"][i].double().view(-1)
+        if "v" in s:
+            m, v = s["m"][i].double().view(-1), s["v"][i].double().view(-1)
+        else:
+            m, v = (c.double().view(-1) * (z.view(torch.uint8).double() - 127).exp2().repeat_interleave(BLOCK)[:n]
+                    for c, z in ((s["m"][i], s["mk"][i]), (s["q"][i], s["qk"][i])))
+            v = v * v
+        m, v = b1 * m + (1 - b1) * g, b2 * v + (1 - b2) * g * g
+        unbiased = (m / (1 - b1 ** t)) / (torch.sqrt(v / (1 - b2 ** t)) + EPS)
+        got["p"][here] = p * (1 - LR * DECAY) - LR * unbiased
+        if "v" in s:
+            got["m"][here], got["v"][here] = m, v
+        else:
+            lo, hi = _random16(n, _key(s["seed"], t, i), g.device)
+            there = slice(at // BLOCK, at // BLOCK + blocks)
+            got["m"][here], got["mk"][there] = _exact_pack(m, lo, False)
+            got["q"][here], got["qk"][there] = _exact_pack(torch.sqrt(v), hi, True)
+        at += blocks * BLOCK
+    return got
