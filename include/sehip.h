@@ -28,7 +28,9 @@
 extern "C" {
 #endif
 
-#define SEHIP_ABI_VERSION 11  /* 11: se_cbn_bwd_ccbam (the CCBAM gate's input gradient formed inside the
+#define SEHIP_ABI_VERSION 12  /* 12: se_layer_norm_fwd / _bwd, se_linear_fwd / _bwd (bias, activation and residual
+                                 in the epilogue), se_adamw_multi (states in 8 or 32 bits);
+                                 11: se_cbn_bwd_ccbam (the CCBAM gate's input gradient formed inside the
                                  encoder CBN backward);
                                  10: 16-bit storage and row biases in se_gemm (the Linear layers), se_bias_grad,
                                  se_copy_strided, the CARN mask / attention-gate / clamp passes, the
@@ -777,6 +779,79 @@ int se_float_to_pcm16(const float* in, long long n, int16_t* out, void* stream);
  * is the windowed-sinc table built by the host (sehip.data.resample_kernel). */
 int se_resample(const float* x, int rows, int L, int orig, int nw, const float* kern, int K, int width,
                 float* out, int Lout, void* stream);
+
+/* ------------------------------------------------------------------------
+ * Layer norm over the last axis (ABI 12; nn.LayerNorm and its autograd).
+ * x: `rows` rows of C elements, x_stride elements apart; y and dx: rows of C.
+ * weight, bias: [C] or NULL (1, 0), of the storage type or fp32 (wdtype).
+ * save: [2][rows] fp32 (mean, 1 / sqrt(var + eps)), written by the forward
+ * (NULL: not wanted) and read by the backward. The backward writes what is not
+ * NULL of dx, dw = sum_r dy h and db = sum_r dy (wdtype; both through ws, added
+ * in a fixed order); variance and all sums in fp32.
+ * ------------------------------------------------------------------------ */
+int se_layer_norm_fwd(const void* x, long long x_stride, long long rows, int C, const void* weight,
+                      const void* bias, float eps, void* y, float* save, int dtype, int wdtype, void* stream);
+size_t se_layer_norm_workspace_size(long long rows, int C);
+int se_layer_norm_bwd(const void* dy, long long dy_stride, const void* x, long long x_stride, long long rows,
+                      int C, const void* weight, const float* save, void* dx, void* dw, void* db, int dtype,
+                      int wdtype, void* ws, size_t ws_bytes, void* stream);
+
+/* ------------------------------------------------------------------------
+ * The product with its epilogue (ABI 12; nn.Linear, an activation and a
+ * residual add): z = x W^T + bias, y = act(z) + residual.
+ * x [M, K] rows ldx apart, w [N, K] rows ldw apart, residual [M, N] rows ldr
+ * apart (or NULL), y and z dense [M, N]; z (or NULL) receives the pre-activation
+ * for the backward. All of one storage type; fp32 accumulation, y rounded once.
+ * Backward: g = dy act'(z) (dy's rows ldr apart), dx = g W, dw = g^T x,
+ * db = sum_m g; what is not NULL is written, z is needed where act is not
+ * SE_LINACT_NONE. The workspace sizes depend on the pointers' alignment.
+ * ------------------------------------------------------------------------ */
+enum {
+  SE_LINACT_NONE = 0,
+  SE_LINACT_RELU = 1,
+  SE_LINACT_GELU = 2,       /* z Phi(z), by erf                                 */
+  SE_LINACT_GELU_TANH = 3,  /* the tanh form                                    */
+  SE_LINACT_SILU = 4
+};
+typedef struct se_linear_desc {
+  int M, N, K;
+  int act, dtype;
+  long long ldx, ldw, ldr;
+} se_linear_desc;
+size_t se_linear_fwd_workspace_size(const se_linear_desc* d, const void* x, const void* w);
+int se_linear_fwd(const se_linear_desc* d, const void* x, const void* w, const void* bias, const void* residual,
+                  void* y, void* z, void* ws, size_t ws_bytes, void* stream);
+size_t se_linear_bwd_workspace_size(const se_linear_desc* d, const void* dy, const void* x, const void* w,
+                                    int want_dx, int want_dw, int want_db);
+int se_linear_bwd(const se_linear_desc* d, const void* dy, const void* x, const void* w, const void* z, void* dx,
+                  void* dw, void* db, void* ws, size_t ws_bytes, void* stream);
+
+/* ------------------------------------------------------------------------
+ * One AdamW step (decoupled decay, amsgrad off) over n tensors (ABI 12), their
+ * table a host array that is read before the call returns.
+ * bits 32: exp_avg and exp_avg_sq are fp32 [numel] whatever the parameters' type.
+ * bits 8: exp_avg holds m and exp_avg_sq holds sqrt(v), each an e4m3 code [numel]
+ * and a scale byte (k + 127 for 2^k) for each SE_ADAMW_BLOCK consecutive
+ * elements, [ceil(numel / SE_ADAMW_BLOCK)]; k is the smallest with
+ * amax <= 448 2^k (at least -126). Rounding is stochastic with 16 bits of a hash
+ * of (seed, step, index of the tensor in the table, element); a positive sqrt(v) is stored as
+ * the smallest code at least; what is not finite is stored as NaN and leaves its
+ * block's scale alone. The parameter moves by m and v before they are rounded and
+ * is itself rounded to nearest.
+ * ------------------------------------------------------------------------ */
+#define SE_ADAMW_BLOCK 128
+typedef struct se_adamw_tensor {
+  void* param;
+  const void* grad;
+  void* exp_avg;
+  void* exp_avg_sq;
+  void* exp_avg_scale;      /* bits 8, else NULL */
+  void* exp_avg_sq_scale;
+  long long numel;
+} se_adamw_tensor;
+int se_adamw_multi(const se_adamw_tensor* tensors, int n, int dtype, int bits, double lr, double beta1,
+                   double beta2, double eps, double weight_decay, long long step, unsigned long long seed,
+                   void* stream);
 
 #ifdef __cplusplus
 }

@@ -8,6 +8,7 @@ torch are then valid inside the library.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import os
 import re
@@ -59,8 +60,15 @@ class GemmDesc(ctypes.Structure):
         (n, c_int) for n in ("kmask_period", "kmask_phase", "splits", "dtype", "bias_rows")]
 
 
+class LinearDesc(ctypes.Structure):
+    """Mirror of se_linear_desc (include/sehip.h, ABI 12)."""
+
+    _fields_ = [(n, c_int) for n in ("M", "N", "K", "act", "dtype")] + [
+        (n, ctypes.c_longlong) for n in ("ldx", "ldw", "ldr")]
+
+
 _P = c_void_p
-ABI_VERSION = 11   # SEHIP_ABI_VERSION (include/sehip.h)
+ABI_VERSION = 12   # SEHIP_ABI_VERSION (include/sehip.h)
 CBN_SAVE_FLOATS = 20   # SE_CBN_SAVE_FLOATS (include/sehip.h)
 _PP = ctypes.POINTER(c_void_p)   # host array of device pointers
 _SIGNATURES = {
@@ -171,6 +179,18 @@ _SIGNATURES = {
     "se_clamp_bwd": (c_int, [_P, _P, _P, ctypes.c_longlong, c_float, c_float, c_int, _P]),
     "se_chunk_split": (c_int, [_P, ctypes.c_longlong, c_int, c_int, c_int, c_int, _P, _P]),
     "se_chunk_overlap_add": (c_int, [_P, c_int, c_int, c_int, c_int, ctypes.c_longlong, c_int, _P, _P]),
+    # ABI 12: layer norm, the product with its epilogue, AdamW with 8- or 32-bit states
+    "se_layer_norm_fwd": (c_int, [_P, ctypes.c_longlong, ctypes.c_longlong, c_int, _P, _P, c_float, _P, _P, c_int,
+                                  c_int, _P]),
+    "se_layer_norm_workspace_size": (c_size_t, [ctypes.c_longlong, c_int]),
+    "se_layer_norm_bwd": (c_int, [_P, ctypes.c_longlong, _P, ctypes.c_longlong, ctypes.c_longlong, c_int, _P, _P, _P,
+                                  _P, _P, c_int, c_int, _P, c_size_t, _P]),
+    "se_linear_fwd_workspace_size": (c_size_t, [_P] * 3),
+    "se_linear_fwd": (c_int, [_P] * 8 + [c_size_t, _P]),
+    "se_linear_bwd_workspace_size": (c_size_t, [_P] * 4 + [c_int] * 3),
+    "se_linear_bwd": (c_int, [_P] * 9 + [c_size_t, _P]),
+    "se_adamw_multi": (c_int, [_P, c_int, c_int, c_int] + [ctypes.c_double] * 5 + [ctypes.c_longlong,
+                                                                                  ctypes.c_ulonglong, _P]),
     "se_complex_join": (c_int, [_P, c_int, c_int, c_int, _P, c_int, c_int, c_int, _P, c_int, c_int, _P]),
     "se_complex_join_bwd": (c_int, [_P, _P, c_int, c_int, c_int, _P, c_int, c_int, c_int, c_int, c_int, _P]),
 }
@@ -221,6 +241,14 @@ def check(rc: int, what: str) -> None:
 def stream_of(t: torch.Tensor) -> int:
     """The caller's current HIP stream for tensor t's device."""
     return torch.cuda.current_stream(t.device).cuda_stream
+
+
+def on_device_of(t: torch.Tensor):
+    """Context in which launches go to t's device (nothing to do where it is the current one)."""
+    return _NOTHING if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
+
+
+_NOTHING = contextlib.nullcontext()
 
 
 def ptr(t) -> int | None:

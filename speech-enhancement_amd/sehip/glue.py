@@ -51,6 +51,20 @@ def copy_into(src: torch.Tensor, dst: torch.Tensor) -> torch.Tensor:
     return dst
 
 
+def as_rows(t: torch.Tensor, C: int, dtype=None):
+    """(t2, ld): t as rows of C contiguous elements ld apart, in `dtype`; copied (se_copy_strided) only where its
+    strides or its type are others. For kernels that read [rows, C] matrices; not differentiable."""
+    if dtype is None or t.dtype == dtype:
+        if t.is_contiguous():
+            return t, C
+        if t.dim() > 1 and (t.stride(-1) == 1 or C == 1):
+            lead = [(n, a) for n, a in zip(t.shape[:-1], t.stride()[:-1]) if n != 1]
+            # rows at one distance: every leading axis spans the ones behind it
+            if not lead or (lead[-1][1] >= C and all(a == b * m for (_, a), (m, b) in zip(lead, lead[1:]))):
+                return t, lead[-1][1] if lead else C
+    return copy_into(t, torch.empty(t.shape, device=t.device, dtype=dtype or t.dtype)), C
+
+
 class _Contig(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, dtype):

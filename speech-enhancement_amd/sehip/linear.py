@@ -20,10 +20,18 @@ With ``halves`` = 2 the input's last axis is split in two equal halves, each
 mapped by its own weight (real_linear on the first, imag_linear on the second),
 the two outputs concatenated on the last axis: ComplexLinear's "no cross terms"
 form (complex_nn.py:106-113) in place, without the chunk / cat.
+
+``linear_act(x, module, act, residual)`` is act(module(x)) + residual with the bias, the
+activation and the residual in the product's epilogue (csrc/linear.hip), from one row (a
+frame of a stream) to a training batch, and its gradients.
 """
 from __future__ import annotations
 
+import ctypes
+
 import torch
+import torch.nn as nn
+from torch.autograd.function import once_differentiable
 
 from . import _native as N
 from . import functional as F
@@ -168,3 +176,106 @@ def linear_halves(x, weights, biases, feature_major_out=False):
 def linear(x, module: torch.nn.Linear, feature_major_out=False):
     """module(x) (nn.Linear) on se_gemm."""
     return linear_halves(x, [module.weight], [module.bias], feature_major_out)
+
+
+ACT_NONE, ACT_RELU, ACT_GELU, ACT_GELU_TANH, ACT_SILU = range(5)   # SE_LINACT_* (include/sehip.h)
+
+
+def _act_code(act) -> int:
+    """SE_LINACT_* of an activation module (an inplace flag makes no difference: z is the kernel's own)."""
+    if act is None or isinstance(act, nn.Identity):
+        return ACT_NONE
+    if isinstance(act, nn.GELU):
+        return ACT_GELU_TANH if act.approximate == "tanh" else ACT_GELU
+    if isinstance(act, nn.SiLU):
+        return ACT_SILU
+    if type(act) is nn.ReLU:
+        return ACT_RELU
+    raise NotImplementedError(f"sehip linear_act: activation {type(act).__name__} (Identity, ReLU, GELU, SiLU)")
+
+
+def _act_forward(x, w, b, res, act, keep):
+    """(y, x as the kernel read it, z); z [M, N] only where `keep` and the activation needs it."""
+    n, k = w.shape
+    m = x.numel() // k
+    y = torch.empty(x.shape[:-1] + (n,), device=x.device, dtype=x.dtype)
+    z = torch.empty((m, n), device=x.device, dtype=x.dtype) if keep and act != ACT_NONE else None
+    x2, ldx = glue.as_rows(x, k)
+    if m:
+        w2, ldw = glue.as_rows(w, k)
+        r2, ldr = (None, n) if res is None else glue.as_rows(res, n)
+        lib = N.lib()
+        d = N.LinearDesc(m, n, k, act, N.DTYPES[x.dtype], ldx, ldw, ldr)
+        p = ctypes.byref(d)
+        xp, wp = x2.data_ptr(), w2.data_ptr()
+        with N.on_device_of(x):
+            need = lib.se_linear_fwd_workspace_size(p, xp, wp)
+            ws = torch.empty(need, device=x.device, dtype=torch.uint8) if need else None
+            N.check(lib.se_linear_fwd(p, xp, wp, N.ptr(b), N.ptr(r2), y.data_ptr(), N.ptr(z), N.ptr(ws), need,
+                                      N.stream_of(x)), "se_linear_fwd")
+    return y, x2, z
+
+
+class _LinearAct(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, w, b, res, act):
+        y, x2, z = _act_forward(x, w, b, res, act, True)
+        ctx.save_for_backward(x2, w, z)
+        ctx.act = act
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, gy):
+        x, w, z = ctx.saved_tensors
+        n, k = w.shape
+        m = x.numel() // k
+        need = ctx.needs_input_grad
+        new = torch.empty if m else torch.zeros
+        dx = torch.empty(x.shape, device=x.device, dtype=x.dtype) if need[0] else None
+        dw = new((n, k), device=x.device, dtype=x.dtype) if need[1] else None
+        db = new(n, device=x.device, dtype=x.dtype) if need[2] else None
+        if m and (need[0] or need[1] or need[2]):
+            g2, ldg = glue.as_rows(gy, n, x.dtype)
+            ldx, (w2, ldw) = glue.as_rows(x, k)[1], glue.as_rows(w, k)
+            lib = N.lib()
+            d = N.LinearDesc(m, n, k, ctx.act, N.DTYPES[x.dtype], ldx, ldw, ldg)
+            p = ctypes.byref(d)
+            gp, xp, wp = g2.data_ptr(), x.data_ptr(), w2.data_ptr()
+            with N.on_device_of(x):
+                size = lib.se_linear_bwd_workspace_size(p, gp, xp, wp, need[0], need[1], need[2])
+                ws = torch.empty(size, device=x.device, dtype=torch.uint8) if size else None
+                N.check(lib.se_linear_bwd(p, gp, xp, wp, N.ptr(z), N.ptr(dx), N.ptr(dw), N.ptr(db), N.ptr(ws), size,
+                                          N.stream_of(x)), "se_linear_bwd")
+        return dx, dw, db, gy if need[3] else None, None
+
+
+def linear_act(x: torch.Tensor, module: nn.Linear, act: nn.Module | None = None,
+               residual: torch.Tensor | None = None) -> torch.Tensor:
+    """act(module(x)) + residual in one product: x [..., in], residual [..., out] (or None), all on one GPU in one of
+    fp32 (each operand split into two scaled fp16 planes, fp32-class), bf16 and fp16 (exact products, fp32 sums, one
+    rounding of the result). act: nn.Identity / None, nn.ReLU, nn.GELU (both forms) or nn.SiLU. For the backward the
+    pre-activation is kept in the storage type. In fp32 an infinity or NaN in x or W makes what it reaches infinite or
+    NaN, not always the one of the two that fp32 products would give. A second derivative is refused."""
+    code = _act_code(act)
+    w, b = module.weight, module.bias
+    for t in (x, w, b, residual):
+        if t is None:
+            continue
+        if not t.is_cuda or t.device != x.device:
+            raise RuntimeError("sehip linear_act: all tensors must be on one GPU (there is no CPU fallback)")
+        if t.dtype != x.dtype or t.dtype not in N.DTYPES:
+            raise RuntimeError(f"sehip linear_act: {t.dtype} beside a {x.dtype} input (one of fp32, bf16, fp16 throughout)")
+    n, k = w.shape
+    if n == 0 or k == 0 or x.dim() == 0 or x.shape[-1] != k:
+        raise RuntimeError(f"sehip linear_act: input {tuple(x.shape)}, weight {tuple(w.shape)}")
+    if residual is not None and residual.shape != x.shape[:-1] + (n,):
+        raise RuntimeError(f"sehip linear_act: residual {tuple(residual.shape)}, output {tuple(x.shape[:-1]) + (n,)} (it is "
+                           "not broadcast)")
+    if b is not None and not b.is_contiguous():
+        raise RuntimeError("sehip linear_act: the bias must be contiguous")
+    LINEAR_CALLS[0] += 1
+    if torch.is_grad_enabled() and (x.requires_grad or w.requires_grad or (b is not None and b.requires_grad)
+                                    or (residual is not None and residual.requires_grad)):
+        return _LinearAct.apply(x, w, b, residual, code)
+    return _act_forward(x, w, b, residual, code, False)[0]

@@ -7,13 +7,21 @@ nn.ELU (constructor, parameters, buffers and state_dict keys unchanged);
 backward (training: batch statistics and the running-stat update as
 nn.BatchNorm2d with a float momentum; eval: running statistics).
 Configurations the kernels do not cover (momentum=None, non-4-D input, other
-activations) run the modules themselves."""
+activations) run the modules themselves.
+
+``layer_norm(norm, x)`` replaces ``norm(x)`` of an nn.LayerNorm, forward and
+backward (csrc/layernorm.hip): any leading shape, rows at any distance, fp32 / bf16 /
+fp16 storage with the weight and bias in the same type or in fp32, the weight's and
+bias's gradients summed in a fixed order. CPU tensors raise."""
 from __future__ import annotations
 
 import torch
 import torch.nn as nn
+from torch.autograd.function import once_differentiable
 
 from . import _native as N
+from . import functional as F
+from . import glue
 
 _ACT_NONE, _ACT_PRELU, _ACT_ELU = 0, 1, 2
 
@@ -96,3 +104,90 @@ def bn_act(norm: nn.Module, act: nn.Module, x: torch.Tensor) -> torch.Tensor:
         norm.num_batches_tracked.add_(1)
     return _BnAct.apply(x, norm.weight, norm.bias, param, rmean, rvar, use_batch, norm.momentum or 0.0, norm.eps,
                         code, param is not None and param.numel() > 1, alpha)
+
+
+def _ln_forward(x, C, weight, bias, eps, keep):
+    """(y, rows of x as the kernel read them, save) of one launch; save None unless `keep`."""
+    x2, ld = glue.as_rows(x, C)
+    rows = x.numel() // C
+    y = torch.empty(x.shape, device=x.device, dtype=x.dtype)
+    save = torch.empty((2, rows), device=x.device, dtype=torch.float32) if keep else None
+    if rows:
+        wt = weight if weight is not None else bias if bias is not None else x
+        with N.on_device_of(x):
+            N.check(N.lib().se_layer_norm_fwd(x2.data_ptr(), ld, rows, C, N.ptr(weight), N.ptr(bias), eps, y.data_ptr(),
+                                              N.ptr(save), N.DTYPES[x.dtype], N.DTYPES[wt.dtype], N.stream_of(x)),
+                    "se_layer_norm_fwd")
+    return y, x2, save
+
+
+class _LayerNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, C, eps):
+        y, x2, save = _ln_forward(x, C, weight, bias, eps, True)
+        ctx.save_for_backward(x2, weight, save)
+        ctx.cfg = (C, None if bias is None else bias.dtype)
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, gy):
+        x, weight, save = ctx.saved_tensors
+        C, bdt = ctx.cfg
+        need = ctx.needs_input_grad
+        rows = x.numel() // C
+        wdt = weight.dtype if weight is not None else bdt or x.dtype
+        dx = torch.empty(x.shape, device=x.device, dtype=x.dtype) if need[0] else None
+        new = torch.empty if rows else torch.zeros
+        dw = new(C, device=x.device, dtype=wdt) if need[1] else None
+        db = new(C, device=x.device, dtype=wdt) if need[2] else None
+        if rows:
+            g2, ldg = glue.as_rows(gy, C, x.dtype)
+            ldx = glue.as_rows(x, C)[1]
+            lib = N.lib()
+            with N.on_device_of(x):
+                ws = F._workspace(lib.se_layer_norm_workspace_size(rows, C), x.device) if need[1] or need[2] else None
+                N.check(lib.se_layer_norm_bwd(g2.data_ptr(), ldg, x.data_ptr(), ldx, rows, C, N.ptr(weight),
+                                              save.data_ptr(), N.ptr(dx), N.ptr(dw), N.ptr(db), N.DTYPES[x.dtype],
+                                              N.DTYPES[wdt], N.ptr(ws), 0 if ws is None else ws.numel(),
+                                              N.stream_of(x)), "se_layer_norm_bwd")
+        if weight is not None:
+            dw = None if dw is None else dw.view(weight.shape)
+            db = None if db is None else db.view(weight.shape)
+        return dx, dw, db, None, None
+
+
+def layer_norm(norm: nn.LayerNorm, x: torch.Tensor) -> torch.Tensor:
+    """norm(x) on the HIP kernels: x [..., *norm.normalized_shape] on the GPU in fp32, bf16 or fp16; norm's weight
+    and bias (each may be absent) both in x's type or both in fp32. The result is contiguous, in x's type. A second
+    derivative is refused."""
+    shape, w, b = norm.normalized_shape, norm.weight, norm.bias
+    k = len(shape)
+    if tuple(x.shape[x.dim() - k:]) != tuple(shape) or x.dim() < k:
+        raise RuntimeError(f"sehip layer_norm: input {tuple(x.shape)} does not end in {tuple(shape)}")
+    for t in (x, w, b):
+        if t is not None and (not t.is_cuda or t.device != x.device):
+            raise RuntimeError("sehip layer_norm: x, weight and bias must be on one GPU (there is no CPU fallback)")
+    if x.dtype not in N.DTYPES:
+        raise RuntimeError(f"sehip layer_norm: unsupported storage type {x.dtype} (fp32, bf16, fp16)")
+    wdt = {t.dtype for t in (w, b) if t is not None}
+    if len(wdt) > 1 or not wdt <= {x.dtype, torch.float32}:
+        raise RuntimeError(f"sehip layer_norm: weight and bias {sorted(map(str, wdt))} beside a {x.dtype} input (both in "
+                           "its type or both in fp32)")
+    C = 1
+    for n in shape:
+        C *= n
+    if C == 0:
+        raise RuntimeError("sehip layer_norm: normalised over no elements")
+    if k > 1:
+        if not all(t is None or t.is_contiguous() for t in (w, b)):
+            raise RuntimeError("sehip layer_norm: weight and bias must be contiguous")
+        return _layer_norm(x.flatten(x.dim() - k), w, b, C, float(norm.eps)).view(x.shape)
+    return _layer_norm(x, w, b, C, float(norm.eps))
+
+
+def _layer_norm(x, w, b, C, eps):
+    if torch.is_grad_enabled() and (x.requires_grad or (w is not None and w.requires_grad)
+                                    or (b is not None and b.requires_grad)):
+        return _LayerNorm.apply(x, w, b, C, eps)
+    return _ln_forward(x, C, w, b, eps, False)[0]

@@ -11,6 +11,11 @@ total norm as a device tensor. Both need contiguous CUDA tensors of one
 storage type per call: fp32, or the bf16 / fp16 of a model.to(bfloat16) /
 .half() run (ABI 10: torch's foreach AdamW rounding reproduced in the kernel).
 There is no CPU path.
+
+``AdamW(..., state_bits=32)`` keeps both moments in fp32 whatever the parameters' type,
+``state_bits=8`` keeps m and sqrt(v) in one byte an element with a power of two for each 128
+(csrc/adamw.hip: the table of tensors travels in the kernel's arguments, 48 a launch).
+``adamw32_`` and ``adamw8_`` are the same steps on tensors in hand.
 """
 from __future__ import annotations
 
@@ -82,15 +87,54 @@ class AdamW(torch.optim.Optimizer):
     count). Parameters of a group normally share their step count; one that
     missed steps (no gradient on some iterations, or a loaded state_dict with
     per-parameter steps) is updated by its own launch with its own bias
-    corrections, as torch tracks the step per parameter."""
+    corrections, as torch tracks the step per parameter.
+
+    state_bits None: the moments in the parameters' type (torch's state layout). 32: state[p] =
+    {'step', 'exp_avg', 'exp_avg_sq'} with fp32 moments. 8: {'step', 'exp_avg', 'exp_avg_scale',
+    'exp_avg_root', 'exp_avg_root_scale'}, e4m3 values of m and sqrt(v) and their e8m0 powers of two,
+    rounded stochastically from `seed`: the replicas of a data-parallel run, given one seed and the same
+    gradients, keep the same states."""
 
     def __init__(self, params, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2, amsgrad=False,
-                 *, maximize=False, foreach=None, capturable=False, differentiable=False, fused=None):
+                 *, maximize=False, foreach=None, capturable=False, differentiable=False, fused=None,
+                 state_bits=None, seed=0):
         if amsgrad or maximize or capturable or differentiable:
             raise NotImplementedError("sehip AdamW: amsgrad / maximize / capturable / differentiable")
         defaults = dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, amsgrad=False, maximize=False,
                         foreach=None, capturable=False, differentiable=False, fused=None)
+        if state_bits is not None:
+            if state_bits not in (8, 32):
+                raise ValueError(f"sehip AdamW: state_bits {state_bits!r} (None, 8 or 32)")
+            defaults.update(state_bits=int(state_bits), seed=int(seed))
         super().__init__(params, defaults)
+
+    def load_state_dict(self, state_dict):
+        """As torch's, but the moments of state_bits 8 / 32 keep their own type (torch casts a state to its
+        parameter's). A state without the keys or types of this optimizer's state_bits is refused, except that
+        state_bits 32 takes moments of any floating type."""
+        given = state_dict["state"]
+        ids = [i for g in state_dict["param_groups"] for i in g["params"]]
+        mine = [(p, g.get("state_bits")) for g in self.param_groups for p in g["params"]]
+        if len(ids) != len(mine):   # torch says which group differs
+            return super().load_state_dict(state_dict)
+        keep = []
+        for i, (p, bits) in zip(ids, mine):
+            if bits is None or i not in given:
+                continue
+            keep.append((p, "step", torch.as_tensor(given[i]["step"]).clone()))
+            want = _state_like(p, bits)
+            for key, like in want.items():
+                t = given[i].get(key)
+                if t is None or t.shape != like.shape or (t.dtype != like.dtype if bits == 8 else not t.is_floating_point()):
+                    raise ValueError(f"sehip AdamW: the loaded state has no {key} for state_bits={bits}")
+                keep.append((p, key, t.to(device=p.device, dtype=like.dtype, copy=True)))
+        own = [{k: g[k] for k in ("state_bits", "seed") if k in g} for g in self.param_groups]
+        super().load_state_dict(state_dict)
+        for g, o in zip(self.param_groups, own):   # the layout of the state is this optimizer's, not the file's
+            g.pop("state_bits", None)
+            g.update({**o, **({"seed": g["seed"]} if "seed" in o and "seed" in g else {})})
+        for p, key, t in keep:
+            self.state[p][key] = t
 
     @torch.no_grad()
     def step(self, closure=None):
@@ -98,7 +142,10 @@ class AdamW(torch.optim.Optimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
-        for group in self.param_groups:
+        for at, group in enumerate(self.param_groups):
+            if group.get("state_bits") is not None:
+                self._step_multi(at, group)
+                continue
             by_step: dict = {}
             for p in group["params"]:
                 if p.grad is None:
@@ -125,3 +172,102 @@ class AdamW(torch.optim.Optimizer):
                                                   float(b2), float(group["eps"]), float(group["weight_decay"]),
                                                   step_val, code, N.stream_of(rs[0][0])), "se_adamw_step")
         return loss
+
+    def _step_multi(self, at, group):
+        bits = group["state_bits"]
+        calls: dict = {}
+        for p in group["params"]:
+            if p.grad is None:
+                continue
+            if p.grad.is_sparse:
+                raise RuntimeError("sehip AdamW: sparse gradients")
+            st = self.state[p]
+            if len(st) == 0:
+                st["step"] = torch.tensor(0.0)
+                st.update(_state_like(p, bits, torch.zeros))
+            calls.setdefault((int(st["step"].item()) + 1, p.dtype, p.device), []).append(p)
+        kw = dict(lr=group["lr"], betas=group["betas"], eps=group["eps"], weight_decay=group["weight_decay"])
+        for (step, _, _), ps in sorted(calls.items(), key=lambda c: c[0][0]):
+            sts = [self.state[p] for p in ps]
+            states = [[st[k] for st in sts] for k in _STATE_KEYS[bits]]
+            if bits == 8:   # a group's own stream of random bits
+                adamw8_(ps, [p.grad for p in ps], *states, step=step, seed=group["seed"] + 0x10001 * at, **kw)
+            else:
+                adamw32_(ps, [p.grad for p in ps], *states, step=step, **kw)
+            for st in sts:   # counted once the launch has gone through
+                st["step"] += 1
+
+
+SCALE_BLOCK = 128   # SE_ADAMW_BLOCK (include/sehip.h)
+_STATE_KEYS = {32: ("exp_avg", "exp_avg_sq"),
+               8: ("exp_avg", "exp_avg_scale", "exp_avg_root", "exp_avg_root_scale")}
+_F8, _E8 = torch.float8_e4m3fn, torch.float8_e8m0fnu
+
+
+def _state_like(p, bits, new=torch.empty):
+    """The moments of a parameter: what AdamW keeps for it (new = torch.zeros), or their shapes and types."""
+    if new is torch.empty:
+        p = torch.empty(p.shape, device="meta")
+    if bits == 32:
+        return {k: new(p.shape, device=p.device, dtype=torch.float32) for k in _STATE_KEYS[32]}
+    blocks = -(-p.numel() // SCALE_BLOCK)
+    return {k: new(blocks if k.endswith("scale") else p.shape, device=p.device, dtype=torch.uint8).view(
+        _E8 if k.endswith("scale") else _F8) for k in _STATE_KEYS[8]}
+
+
+_TENSOR = np.dtype([("param", "<u8"), ("grad", "<u8"), ("exp_avg", "<u8"), ("exp_avg_sq", "<u8"),
+                    ("exp_avg_scale", "<u8"), ("exp_avg_sq_scale", "<u8"), ("numel", "<i8")])   # se_adamw_tensor
+
+
+def _multi(params, columns, types, bits, step, lr, betas, eps, weight_decay, seed):
+    """se_adamw_multi over `params` and the columns grad, exp_avg, exp_avg_sq (, their scales)."""
+    n = len(params)
+    if any(len(c) != n for c in columns):
+        raise ValueError("sehip adamw: lists of different lengths")
+    if n == 0:
+        return
+    if step < 1:
+        raise ValueError(f"sehip adamw: step {step} (counted from 1)")
+    if not (0.0 <= betas[0] < 1.0 and 0.0 <= betas[1] < 1.0):
+        raise ValueError(f"sehip adamw: betas {betas}")
+    p0 = params[0]
+    dev, dt = p0.device, p0.dtype
+    if dev.type != "cuda" or dt not in N.DTYPES:
+        raise RuntimeError("sehip adamw: parameters must be fp32, bf16 or fp16 CUDA tensors (there is no CPU path)")
+    sizes = [p.numel() for p in params]
+    blocks = [-(-k // SCALE_BLOCK) for k in sizes] if bits == 8 else None
+    arr = np.zeros(n, dtype=_TENSOR)
+    for name, ts, ty in zip(_TENSOR.names, (params, *columns), (dt, *types)):
+        want = blocks if name.endswith("scale") else sizes
+        for t, k in zip(ts, want):
+            if t.dtype != ty or t.numel() != k or not t.is_contiguous() or t.device != dev:
+                raise RuntimeError(f"sehip adamw: {name} of {t.numel()} {t.dtype} on {t.device}, expected {k} contiguous {ty} "
+                                   f"on {dev}")
+        arr[name] = [t.data_ptr() for t in ts]
+    arr["numel"] = sizes
+    if torch.cuda.is_current_stream_capturing():
+        raise RuntimeError("sehip adamw: a captured graph would repeat this step's count and bias corrections")
+    with N.on_device_of(p0):
+        N.check(N.lib().se_adamw_multi(arr.ctypes.data, n, N.DTYPES[dt], bits, float(lr), float(betas[0]), float(betas[1]),
+                                       float(eps), float(weight_decay), int(step), int(seed) & 0xFFFFFFFFFFFFFFFF,
+                                       N.stream_of(p0)), "se_adamw_multi")
+    written = [*params, *columns[1], *columns[2]]
+    torch.autograd.graph.increment_version(written)
+
+
+@torch.no_grad()
+def adamw32_(params, grads, exp_avgs, exp_avg_sqs, *, step, lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2):
+    """One AdamW step in place over lists of contiguous tensors on one GPU: parameters and gradients of one type
+    (fp32, bf16, fp16), moments in fp32. step counts from 1."""
+    _multi(params, (grads, exp_avgs, exp_avg_sqs), (params[0].dtype if params else None, torch.float32, torch.float32), 32,
+           step, lr, betas, eps, weight_decay, 0)
+
+
+@torch.no_grad()
+def adamw8_(params, grads, exp_avgs, exp_avg_scales, roots, root_scales, *, step, lr=1e-3, betas=(0.9, 0.999), eps=1e-8,
+            weight_decay=1e-2, seed=0):
+    """One AdamW step in place whose moments are held in 8 bits: exp_avgs and roots (m and sqrt(v)) float8_e4m3fn of
+    the parameters' shapes, the scales float8_e8m0fnu [ceil(numel / 128)]. m and v are rounded stochastically with a hash of
+    (seed, step, place in the list, element): the same call gives the same bits."""
+    _multi(params, (grads, exp_avgs, roots, exp_avg_scales, root_scales),
+           (params[0].dtype if params else None, _F8, _F8, _E8, _E8), 8, step, lr, betas, eps, weight_decay, seed)
