@@ -19,6 +19,8 @@
 #include "common.hpp"
 
 #include <algorithm>
+#include <cmath>
+#include <type_traits>
 
 namespace {
 
@@ -40,7 +42,7 @@ struct Epi {
   const void* res;      // [M][N] at ldr, or NULL
   const short* ea;      // power of two of each row of A and of B (fp32), or NULL
   const short* eb;
-  long long ldc, ldr;   // z has rows of N
+  long long ldc, ldr, ldz;
   int act;
 };
 
@@ -57,86 +59,143 @@ struct GemmArgs {
   Epi e;
 };
 
-__device__ __forceinline__ float act_of(int act, float z) {
-  switch (act) {
-    case SE_LINACT_RELU: return z > 0.f ? z : (z == z ? 0.f : z);
-    case SE_LINACT_GELU: return 0.5f * z * (1.f + erff(z * 0.70710678118654752f));
-    case SE_LINACT_GELU_TANH: return 0.5f * z * (1.f + tanhf(0.79788456080286536f * (z + 0.044715f * z * z * z)));
-    case SE_LINACT_SILU: return z / (1.f + expf(-z));
-    default: return z;
-  }
+// The activations by the hardware's exponential and reciprocal (1 ulp each): sigma(t) = 1 / (1 + 2^(-t log2 e)).
+__device__ __forceinline__ float sigmoid_fast(float t) {
+  return __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(-1.4426950408889634f * t));
 }
-
-__device__ __forceinline__ float slope_of(int act, float z) {
-  switch (act) {
-    case SE_LINACT_RELU: return z > 0.f ? 1.f : 0.f;
-    case SE_LINACT_GELU:
-      return 0.5f * (1.f + erff(z * 0.70710678118654752f)) + z * 0.3989422804014327f * expf(-0.5f * z * z);
-    case SE_LINACT_GELU_TANH: {
-      const float t = tanhf(0.79788456080286536f * (z + 0.044715f * z * z * z));
-      return 0.5f * (1.f + t) + 0.5f * z * (1.f - t * t) * 0.79788456080286536f * (1.f + 0.134145f * z * z);
-    }
-    case SE_LINACT_SILU: {
-      const float p = 1.f / (1.f + expf(-z));
-      return p * (1.f + z * (1.f - p));
-    }
-    default: return 1.f;
-  }
-}
-
-// four consecutive columns n .. n + 3 of row m, out of the accumulators or the slabs
-template <typename S>
-__device__ __forceinline__ void epilogue4(const Epi& e, int M, int N, int m, int n, float (&v)[4], bool vec) {
-  struct alignas(4 * sizeof(S)) P { S x[4]; };
-  if (m >= M || n >= N) return;
-  const int left = N - n;
-  if (e.ea) {
-    const int s = e.ea[m] - 2 * kTop;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) v[j] = __builtin_ldexpf(v[j], s + (j < left ? e.eb[n + j] : 0));
-  }
-  const long long o = (long long)m * e.ldc + n, oz = (long long)m * N + n, orr = (long long)m * e.ldr + n;
-  if (e.bias) {
-    const S* b = static_cast<const S*>(e.bias) + n;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) v[j] += j < left ? (float)b[j] : 0.f;
-  }
-  if (vec && left >= 4) {
-    P t;
-    if (e.z) {
-#pragma unroll
-      for (int j = 0; j < 4; ++j) t.x[j] = (S)v[j];
-      *reinterpret_cast<P*>(static_cast<S*>(e.z) + oz) = t;
-    }
-    if (e.act)
-#pragma unroll
-      for (int j = 0; j < 4; ++j) v[j] = act_of(e.act, v[j]);
-    if (e.res) {
-      const P r = *reinterpret_cast<const P*>(static_cast<const S*>(e.res) + orr);
-#pragma unroll
-      for (int j = 0; j < 4; ++j) v[j] += (float)r.x[j];
-    }
-#pragma unroll
-    for (int j = 0; j < 4; ++j) t.x[j] = (S)v[j];
-    *reinterpret_cast<P*>(static_cast<S*>(e.C) + o) = t;
+// Phi(z), and phi(z): for fp32 storage by erf; for 16 bits by Hastings' approximation of erfc (Abramowitz and Stegun 7.1.26),
+// which is 1.5e-7 off at most, far below a step of either type at any z whose Phi is not itself that small
+template <bool FAST>
+__device__ __forceinline__ float normal_cdf(float z, float& phi) {
+  const float e = __builtin_amdgcn_exp2f(-0.72134752044448170f * z * z);   // exp(-z^2 / 2)
+  phi = 0.3989422804014327f * e;
+  if constexpr (FAST) {
+    const float t = __builtin_amdgcn_rcpf(1.f + 0.3275911f * 0.70710678118654752f * fabsf(z));
+    const float q = 0.5f * e * t * (0.254829592f + t * (-0.284496736f + t * (1.421413741f + t * (-1.453152027f + t * 1.061405429f))));
+    return z < 0.f ? q : 1.f - q;
   } else {
+    return z < 0.f ? 0.5f * erfcf(-0.70710678118654752f * z) : 0.5f + 0.5f * erff(0.70710678118654752f * z);
+  }
+}
+// the argument of the tanh form: z (1 + tanh c(z + a z^3)) / 2 = z sigma(2 c (z + a z^3))
+__device__ __forceinline__ float tanh_arg(float z) { return 1.5957691216057308f * (z + 0.044715f * z * z * z); }
+
+template <bool FAST, int V>
+__device__ __forceinline__ void act_of(int act, float (&v)[V]) {
+  switch (act) {   // one branch for the V values
+    case SE_LINACT_RELU:
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      if (j >= left) continue;
-      if (e.z) static_cast<S*>(e.z)[oz + j] = (S)v[j];
-      float r = e.act ? act_of(e.act, v[j]) : v[j];
-      if (e.res) r += (float)static_cast<const S*>(e.res)[orr + j];
-      static_cast<S*>(e.C)[o + j] = (S)r;
-    }
+      for (int j = 0; j < V; ++j) v[j] = v[j] < 0.f ? 0.f : v[j];   // a NaN stays
+      break;
+    case SE_LINACT_GELU:
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        float phi;
+        v[j] *= normal_cdf<FAST>(v[j], phi);
+      }
+      break;
+    case SE_LINACT_GELU_TANH:
+#pragma unroll
+      for (int j = 0; j < V; ++j) v[j] *= sigmoid_fast(tanh_arg(v[j]));
+      break;
+    case SE_LINACT_SILU:
+#pragma unroll
+      for (int j = 0; j < V; ++j) v[j] *= sigmoid_fast(v[j]);
+      break;
+    default: break;
   }
 }
 
-// whether rows of C, z and the residual take four columns in one access
-template <typename S>
+// v *= act'(z)
+template <bool FAST, int V>
+__device__ __forceinline__ void slope_of(int act, const float (&z)[V], float (&v)[V]) {
+  switch (act) {
+    case SE_LINACT_RELU:
+#pragma unroll
+      for (int j = 0; j < V; ++j) v[j] = z[j] <= 0.f ? 0.f : v[j];
+      break;
+    case SE_LINACT_GELU:
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        float phi;
+        const float c = normal_cdf<FAST>(z[j], phi);
+        v[j] *= c + z[j] * phi;
+      }
+      break;
+    case SE_LINACT_GELU_TANH:
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        const float p = sigmoid_fast(tanh_arg(z[j]));
+        v[j] *= p + z[j] * p * (1.f - p) * (1.5957691216057308f * (1.f + 0.134145f * fminf(z[j] * z[j], 1e30f)));
+      }
+      break;
+    case SE_LINACT_SILU:
+#pragma unroll
+      for (int j = 0; j < V; ++j) {
+        const float p = sigmoid_fast(z[j]);
+        v[j] *= p * (1.f + z[j] * (1.f - p));
+      }
+      break;
+    default: break;
+  }
+}
+
+template <typename S, int V> struct alignas(sizeof(S) * V > 16 ? 16 : sizeof(S) * V) Pack { S x[V]; };
+template <typename S, int V>
+__device__ __forceinline__ void load_pack(const S* p, float (&v)[V]) {
+  const Pack<S, V> t = *reinterpret_cast<const Pack<S, V>*>(p);
+#pragma unroll
+  for (int j = 0; j < V; ++j) v[j] = (float)t.x[j];
+}
+template <typename S, int V>
+__device__ __forceinline__ void store_pack(S* p, const float (&v)[V]) {
+  Pack<S, V> t;
+#pragma unroll
+  for (int j = 0; j < V; ++j) t.x[j] = (S)v[j];
+  *reinterpret_cast<Pack<S, V>*>(p) = t;
+}
+
+// what V consecutive columns n .. (all inside) have for every row
+template <typename S, int V>
+struct Cols {
+  float bias[V];
+  int eb[V];
+  __device__ __forceinline__ void load(const Epi& e, int n) {
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      bias[j] = 0.f;
+      eb[j] = 0;
+    }
+    if (e.bias) load_pack<S, V>(static_cast<const S*>(e.bias) + n, bias);
+    if (e.ea)
+#pragma unroll
+      for (int j = 0; j < V; ++j) eb[j] = e.eb[n + j] - 2 * kTop;
+  }
+};
+
+// those columns of row m, out of the sums; res: the residual's values. Every row is aligned for V.
+template <typename S, int V>
+__device__ __forceinline__ void epilogue(const Epi& e, const Cols<S, V>& cols, long long m, int n, float (&v)[V],
+                                         const float (&res)[V], int ea) {
+  if (e.ea)
+#pragma unroll
+    for (int j = 0; j < V; ++j) v[j] = __builtin_ldexpf(v[j], ea + cols.eb[j]);
+#pragma unroll
+  for (int j = 0; j < V; ++j) v[j] += cols.bias[j];
+  if (e.z) store_pack<S, V>(static_cast<S*>(e.z) + m * e.ldz + n, v);
+  act_of<sizeof(S) == 2, V>(e.act, v);
+  if (e.res)
+#pragma unroll
+    for (int j = 0; j < V; ++j) v[j] += res[j];
+  store_pack<S, V>(static_cast<S*>(e.C) + m * e.ldc + n, v);
+}
+
+// whether the rows of C, z, the residual and the bias take V columns in one access (z's rows are laid out for it)
+template <typename S, int V>
 __device__ __forceinline__ bool vec_of(const Epi& e, int N) {
-  const unsigned long long al = 4 * sizeof(S) - 1;
-  return ((unsigned long long)e.C & al) == 0 && e.ldc % 4 == 0 && (!e.z || (N % 4 == 0 && ((unsigned long long)e.z & al) == 0)) &&
-         (!e.res || (((unsigned long long)e.res & al) == 0 && e.ldr % 4 == 0));
+  constexpr unsigned long long al = (sizeof(S) * V > 16 ? 16 : sizeof(S) * V) - 1;
+  return N % V == 0 && (((unsigned long long)e.C | (unsigned long long)e.bias | (unsigned long long)e.res) & al) == 0 &&
+         e.ldc % V == 0 && (!e.res || e.ldr % V == 0);
 }
 
 typedef __attribute__((address_space(3))) void* lds_ptr;
@@ -162,21 +221,17 @@ struct Tile {
   // k of this lane's chunk within the tile (KC)
   static __device__ __forceinline__ int lane_k(int lane) { return ((lane & 7) ^ (lane >> 3)) * 8; }
 
-  static __device__ __forceinline__ void load(const u16* base, long long at, long long bytes, long long ld, int kleft,
-                                              unsigned off, int lane, int wave, u16* lds) {
+  // the matrix from element `at` on, `bytes` in all: reads behind its end give zeros
+  static __device__ __forceinline__ __amdgpu_buffer_rsrc_t source(const u16* base, long long at, long long bytes) {
     const long long left = bytes - at * 2;
     const int rec = left <= 0 ? 0 : (int)(left < 0x7ffffff0LL ? left : 0x7ffffff0LL);
-    const __amdgpu_buffer_rsrc_t r =
-        __builtin_amdgcn_make_buffer_rsrc(se::uniform_ptr(base + at), (short)0, __builtin_amdgcn_readfirstlane(rec), 0x00020000);
-    if constexpr (KC)
-      if (kleft < kBK && lane_k(lane) >= kleft) off = 0x80000000u;   // behind the row's end: zeros
-#pragma unroll
-    for (int q = 0; q < kInstr; ++q) {
-      const int i = q * NW + wave;
-      const int so = (int)((KC ? 8 : kRowsRC) * ld * 2) * i;
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_ptr)(lds + i * 512), 16, (int)off,
-                                               __builtin_amdgcn_readfirstlane(so), 0, 0);
-    }
+    return __builtin_amdgcn_make_buffer_rsrc(se::uniform_ptr(base + at), (short)0, __builtin_amdgcn_readfirstlane(rec), 0x00020000);
+  }
+  // wave load q of kInstr: 1 KB of the tile
+  static __device__ __forceinline__ void load(__amdgpu_buffer_rsrc_t r, unsigned off, int ld, int wave, int q, u16* lds) {
+    const int i = q * NW + wave;
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(r, (lds_ptr)(lds + i * 512), 16, (int)off,
+                                             __builtin_amdgcn_readfirstlane((KC ? 8 : kRowsRC) * 2 * i * ld), 0, 0);
   }
 
   // this lane's eight k (kk + 8 (lane / 32) ..) of row f0 + (lane & 31)
@@ -217,9 +272,48 @@ __device__ __forceinline__ void tile_of(int id, int MT, int NT, int& mt, int& nt
   nt = in / deep;
 }
 
+// 32 rows of TN sums from `turn` through the epilogue (or into the slab), V columns a lane: the rows' residuals of four
+// turns are asked for together
+template <typename S, int V, int TN, int PITCH>
+__device__ __forceinline__ void drain(const GemmArgs& a, float* slab, const float* turn, int lane, int mb, int nb) {
+  constexpr int kWide = TN < 64 * V ? TN : 64 * V, kLanes = kWide / V, kRows = 64 / kLanes, kU = 32 / kRows < 4 ? 32 / kRows : 4;
+#pragma unroll 1
+  for (int c = (lane % kLanes) * V; c < TN; c += kWide) {
+    const int n = nb + c;
+    if (n >= a.N) continue;   // V divides N
+    Cols<S, V> cols;
+    if (!slab) cols.load(a.e, n);
+#pragma unroll 1
+    for (int r0 = lane / kLanes; r0 < 32; r0 += kU * kRows) {
+      float res[kU][V];
+      int ea[kU];
+#pragma unroll
+      for (int u = 0; u < kU; ++u) {
+        const int m = mb + r0 + u * kRows;
+#pragma unroll
+        for (int k = 0; k < V; ++k) res[u][k] = 0.f;
+        ea[u] = 0;
+        if (m >= a.M || slab) continue;
+        if (a.e.res) load_pack<S, V>(static_cast<const S*>(a.e.res) + m * a.e.ldr + n, res[u]);
+        if (a.e.ea) ea[u] = a.e.ea[m];
+      }
+#pragma unroll
+      for (int u = 0; u < kU; ++u) {
+        const int r = r0 + u * kRows, m = mb + r;
+        if (m >= a.M) continue;
+        float v[V];
+        load_pack<float, V>(turn + r * PITCH + c, v);
+        if (slab) store_pack<float, V>(slab + (long long)m * a.N + n, v);
+        else epilogue<S, V>(a.e, cols, m, n, v, res[u], ea[u]);
+      }
+    }
+  }
+}
+
 // H: the products' type; S: the storage type of C, z, bias and residual (H, or float)
 template <typename H, typename S, bool AKC, bool BKC, int BM, int BN, int WM, int WN>
-__global__ void __launch_bounds__(WM * WN * 64, 2) linear_gemm_kernel(const GemmArgs a) {
+__global__ void __launch_bounds__(WM * WN * 64, BM == 256 && WM * WN == 4 ? 1 : 2) linear_gemm_kernel(const GemmArgs a) {
+  constexpr int kTerms = __is_same(S, float) ? 3 : 1;
   constexpr int NW = WM * WN, TM = BM / WM, TN = BN / WN, FM = TM / 32, FN = TN / 32;
   using TA = Tile<AKC, BM, NW>;
   using TB = Tile<BKC, BN, NW>;
@@ -233,13 +327,28 @@ __global__ void __launch_bounds__(WM * WN * 64, 2) linear_gemm_kernel(const Gemm
   const int s0 = blockIdx.y * a.per, s1 = min(a.steps, s0 + a.per);
   const unsigned offA = TA::lane_offset(lane, wave, a.lda), offB = TB::lane_offset(lane, wave, a.ldb);
 
-  auto load = [&](int s, u16* la, u16* lb) __attribute__((always_inline)) {
-    const int term = s / a.ksteps, k0 = (s - term * a.ksteps) * kBK, kleft = a.K - k0;
-    const u16* pa = a.A[term == 2];
-    const u16* pb = a.B[term == 1];
-    TA::load(pa, AKC ? m0 * a.lda + k0 : k0 * a.lda + m0, a.a_bytes, a.lda, kleft, offA, lane, wave, la);
-    TB::load(pb, BKC ? n0 * a.ldb + k0 : k0 * a.ldb + n0, a.b_bytes, a.ldb, kleft, offB, lane, wave, lb);
-    __builtin_amdgcn_sched_barrier(0);   // the scheduler would sink the loads to the barrier that waits for them
+  // where the tile after the one that is being loaded lies: its sources, and the lanes' offsets into them
+  struct Next {
+    __amdgpu_buffer_rsrc_t a, b;
+    unsigned oa, ob;
+  } next;
+  auto aim = [&](int s) __attribute__((always_inline)) {
+    const int term = kTerms == 1 ? 0 : s / a.ksteps, k0 = (s - term * a.ksteps) * kBK, kleft = a.K - k0;
+    const bool on = s < s1;   // behind the last one: nothing is read
+    next.a = TA::source(a.A[term == 2], AKC ? m0 * a.lda + k0 : k0 * a.lda + m0, on ? a.a_bytes : 0);
+    next.b = TB::source(a.B[term == 1], BKC ? n0 * a.ldb + k0 : k0 * a.ldb + n0, on ? a.b_bytes : 0);
+    // KC, behind the row's end: zeros
+    next.oa = AKC && kleft < kBK && TA::lane_k(lane) >= kleft ? 0x80000000u : offA;
+    next.ob = BKC && kleft < kBK && TB::lane_k(lane) >= kleft ? 0x80000000u : offB;
+  };
+  constexpr int kLoads = TA::kInstr + TB::kInstr;
+  auto load = [&](int from, int to, u16* la, u16* lb) __attribute__((always_inline)) {
+#pragma unroll
+    for (int q = 0; q < kLoads; ++q) {
+      if (q < from || q >= to) continue;
+      if (q < TA::kInstr) TA::load(next.a, next.oa, (int)a.lda, wave, q, la);
+      else TB::load(next.b, next.ob, (int)a.ldb, wave, q - TA::kInstr, lb);
+    }
   };
 
   f32x16 acc[FN][FM];
@@ -250,94 +359,140 @@ __global__ void __launch_bounds__(WM * WN * 64, 2) linear_gemm_kernel(const Gemm
 #pragma unroll
       for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.f;
 
-  auto compute = [&](const u16* la, const u16* lb) __attribute__((always_inline)) {
+  // The fragments of the next sixteen k are read while the matrix unit works on these; the last sixteen of a tile come
+  // after the barrier that opens the next tile, so that its first fragments, and the loads into the tile just left,
+  // are under way meanwhile.
+  s16x8 fa[2][FM], fb[2][FN];
+  auto read = [&](int set, const u16* la, const u16* lb, int kk) __attribute__((always_inline)) {
 #pragma unroll
-    for (int kk = 0; kk < kBK; kk += 16) {
-      s16x8 fa[FM], fb[FN];
+    for (int i = 0; i < FN; ++i) fb[set][i] = TB::fragment(lb, wn + 32 * i, kk, lane);
 #pragma unroll
-      for (int j = 0; j < FM; ++j) fa[j] = TA::fragment(la, wm + 32 * j, kk, lane);
+    for (int j = 0; j < FM; ++j) fa[set][j] = TA::fragment(la, wm + 32 * j, kk, lane);
+  };
+  auto multiply = [&](int set) __attribute__((always_inline)) {
 #pragma unroll
-      for (int i = 0; i < FN; ++i) fb[i] = TB::fragment(lb, wn + 32 * i, kk, lane);
+    for (int j = 0; j < FM; ++j)
+#pragma unroll
+      for (int i = 0; i < FN; ++i) acc[i][j] = mfma<H>(fb[set][i], fa[set][j], acc[i][j]);
+  };
+  // LDS reads and loads between the products: all waves ask at the same time, and a wave whose requests wait their turn in
+  // front of its products would start those late.
+  auto mixed = [&](auto loads) __attribute__((always_inline)) {
+    constexpr int kReads = FM * (AKC ? 1 : 2) + FN * (BKC ? 1 : 2), kProducts = FM * FN, kV = decltype(loads)::value;
+    constexpr int kEach = (kReads + kProducts - 1) / kProducts;
+#pragma unroll
+    for (int i = 0; i < kProducts; ++i) {
+      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);                               // a product
+      if (i * kEach < kReads) __builtin_amdgcn_sched_group_barrier(0x100, kEach, 0);   // LDS reads
+#pragma unroll
+      for (int v = i * kV / kProducts; v < (i + 1) * kV / kProducts; ++v)
+        __builtin_amdgcn_sched_group_barrier(0x010, 1, 0);   // a load
+    }
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  // The loads of a tile: the first part right after the barrier that frees its buffer, the rest over the next two steps, so
+  // that the last of them has a step's time until the barrier that waits for it.
+  constexpr int kL0 = (kLoads + 2) / 3, kL1 = kL0 + (kLoads - kL0 + 1) / 2;
+  using N0 = std::integral_constant<int, kL0>;
+  using N1 = std::integral_constant<int, kL1 - kL0>;
+  using N2 = std::integral_constant<int, kLoads - kL1>;
+  // Tile s in (la, lb), its first fragments in set 0; tile s + 1 is on its way to (na, nb), whose first fragments are read at
+  // the end, when the loads of tile s + 2 into (la, lb) begin.
+  auto tile = [&](u16* la, u16* lb, u16* na, u16* nb, int s) __attribute__((always_inline)) {
+    load(kL0, kL1, na, nb);
+    read(1, la, lb, 16);
+    multiply(0);
+    mixed(N1{});
+    load(kL1, kLoads, na, nb);
+    read(0, la, lb, 32);
+    multiply(1);
+    mixed(N2{});
+    read(1, la, lb, 48);
+    multiply(0);
+    mixed(std::integral_constant<int, 0>{});
+    aim(s + 2);
+    __syncthreads();
+    load(0, kL0, la, lb);
+    read(0, na, nb, 0);   // after the last tile nothing uses it
+    multiply(1);
+    mixed(N0{});
+  };
+
+  // two buffers of their own names, so that the compiler sees that a tile's loads do not touch the one being read
+  aim(s0);
+  load(0, kLoads, sA0, sB0);
+  aim(s0 + 1);
+  load(0, kL0, sA1, sB1);
+  __syncthreads();
+  read(0, sA0, sB0, 0);
+  for (int s = s0; s < s1; s += 2) {   // the tile behind an odd number of them is zeros
+    tile(sA0, sB0, sA1, sB1, s);
+    tile(sA1, sB1, sA0, sB0, s + 1);
+  }
+  __syncthreads();
+
+  // The accumulators of block (i, j) hold, in lane l, row m = l & 31 and four consecutive n in each of four groups. Each wave
+  // turns 32 rows at a time through the LDS that the tiles no longer need, so that a row's columns leave side by side:
+  // 16 bytes a lane (a 16-bit row of 64 columns is one 128-byte line) where the rows are aligned for it.
+  constexpr int kPitch = TN + 4, kPer = NW / 4;   // waves to each of the four buffers
+  static_assert(kPer * 32 * kPitch * 4 <= (BM < BN ? BM : BN) * kBK * 2, "the turned rows fit");
+  const int which = wave / kPer;
+  float* turn = reinterpret_cast<float*>(which == 0 ? sA0 : which == 1 ? sB0 : which == 2 ? sA1 : sB1) + (wave % kPer) * 32 * kPitch;
+  float* slab = a.slab ? a.slab + (long long)blockIdx.y * a.M * a.N : nullptr;
+  const int wide = a.slab ? (a.N % 8 == 0 ? 8 : a.N % 2 == 0 ? 2 : 1) : vec_of<S, 8>(a.e, a.N) ? 8 : vec_of<S, 2>(a.e, a.N) ? 2 : 1;
+#pragma unroll 1
+  for (int j = 0; j < FM; ++j) {
+    auto put = [&](auto at) __attribute__((always_inline)) {
+      constexpr int J = decltype(at)::value;
 #pragma unroll
       for (int i = 0; i < FN; ++i)
 #pragma unroll
-        for (int j = 0; j < FM; ++j) acc[i][j] = mfma<H>(fb[i], fa[j], acc[i][j]);
+        for (int q = 0; q < 4; ++q)
+          *reinterpret_cast<f32x4*>(turn + (lane & 31) * kPitch + 32 * i + 8 * q + 4 * (lane >> 5)) =
+              (f32x4){acc[i][J][4 * q], acc[i][J][4 * q + 1], acc[i][J][4 * q + 2], acc[i][J][4 * q + 3]};
+    };
+    static_assert(FM == 1 || FM == 2 || FM == 4, "the blocks below");
+    if (j == 0) put(std::integral_constant<int, 0>{});
+    if constexpr (FM > 1) if (j == 1) put(std::integral_constant<int, 1>{});
+    if constexpr (FM > 2) {
+      if (j == 2) put(std::integral_constant<int, 2>{});
+      if (j == 3) put(std::integral_constant<int, 3>{});
     }
-  };
-
-  if (s0 < s1) {
-    load(s0, sA0, sB0);
-    __syncthreads();
-    int s = s0;
-    for (; s + 2 < s1; s += 2) {
-      load(s + 1, sA1, sB1);
-      compute(sA0, sB0);
-      __syncthreads();
-      load(s + 2, sA0, sB0);
-      compute(sA1, sB1);
-      __syncthreads();
-    }
-    if (s + 1 < s1) {
-      load(s + 1, sA1, sB1);
-      compute(sA0, sB0);
-      __syncthreads();
-      compute(sA1, sB1);
-    } else {
-      compute(sA0, sB0);
-    }
-  }
-
-  // block (i, j): this lane's column of the accumulator is row m, its registers 4 q .. 4 q + 3 four consecutive n
-  const bool vec = vec_of<S>(a.e, a.N);
-  float* slab = a.slab ? a.slab + (long long)blockIdx.y * a.M * a.N : nullptr;
-#pragma unroll
-  for (int j = 0; j < FM; ++j) {
-    const int m = m0 + wm + 32 * j + (lane & 31);
-#pragma unroll
-    for (int i = 0; i < FN; ++i)
-#pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const int n = n0 + wn + 32 * i + 8 * q + 4 * (lane >> 5);
-        float v[4];
-#pragma unroll
-        for (int r = 0; r < 4; ++r) v[r] = acc[i][j][4 * q + r];
-        if (!slab) {
-          epilogue4<S>(a.e, a.M, a.N, m, n, v, vec);
-        } else if (m < a.M) {
-          float* p = slab + (long long)m * a.N + n;
-          if (a.N % 4 == 0 && n < a.N) *reinterpret_cast<f32x4*>(p) = (f32x4){v[0], v[1], v[2], v[3]};
-          else
-#pragma unroll
-            for (int r = 0; r < 4; ++r)
-              if (n + r < a.N) p[r] = v[r];
-        }
-      }
+    __builtin_amdgcn_wave_barrier();   // a wave's LDS accesses are in order; the compiler's must be too
+    const int mb = m0 + wm + 32 * j;
+    if (wide == 8) drain<S, 8, TN, kPitch>(a, slab, turn, lane, mb, n0 + wn);
+    else if (wide == 2) drain<S, 2, TN, kPitch>(a, slab, turn, lane, mb, n0 + wn);
+    else drain<S, 1, TN, kPitch>(a, slab, turn, lane, mb, n0 + wn);
+    __builtin_amdgcn_wave_barrier();
   }
 }
 
-// the slabs of a split product, added in order, and the epilogue
-template <typename S>
+// the slabs of a split product, added in order, and the epilogue: V columns a thread
+template <typename S, int V>
 __global__ void __launch_bounds__(256) linear_join_kernel(const GemmArgs a) {
-  const int N4 = (a.N + 3) / 4;
-  const long long total = (long long)a.M * N4, mn = (long long)a.M * a.N;
-  const bool vec = vec_of<S>(a.e, a.N), whole = a.N % 4 == 0;
+  const int NV = a.N / V;
+  const long long total = (long long)a.M * NV, mn = (long long)a.M * a.N;
   for (long long i = blockIdx.x * 256LL + threadIdx.x; i < total; i += gridDim.x * 256LL) {
-    const int m = (int)(i / N4), n = (int)(i - (long long)m * N4) * 4;
-    const float* p = a.slab + (long long)m * a.N + n;
-    float v[4] = {0.f, 0.f, 0.f, 0.f};
-    if (whole) {
-      for (int s = 0; s < a.splits; ++s) {
-        const f32x4 t = *reinterpret_cast<const f32x4*>(p + s * mn);
+    const long long m = i / NV;
+    const int n = (int)(i - m * NV) * V;
+    const float* p = a.slab + m * a.N + n;
+    float v[V];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) v[j] += t[j];
-      }
-    } else {
-      for (int s = 0; s < a.splits; ++s)
+    for (int j = 0; j < V; ++j) v[j] = 0.f;
+#pragma unroll 4
+    for (int s = 0; s < a.splits; ++s) {
+      float t[V];
+      load_pack<float, V>(p + s * mn, t);
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-          if (n + j < a.N) v[j] += p[s * mn + j];
+      for (int j = 0; j < V; ++j) v[j] += t[j];
     }
-    epilogue4<S>(a.e, a.M, a.N, m, n, v, vec);
+    Cols<S, V> cols;
+    cols.load(a.e, n);
+    float res[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) res[j] = 0.f;
+    if (a.e.res) load_pack<S, V>(static_cast<const S*>(a.e.res) + m * a.e.ldr + n, res);
+    epilogue<S, V>(a.e, cols, m, n, v, res, a.e.ea ? a.e.ea[m] : 0);
   }
 }
 
@@ -421,30 +576,52 @@ __global__ void __launch_bounds__(256) linear_split_cols_kernel(const float* __r
 }
 
 // g = dy act'(z) in rows of Np (zeros behind N), and each chunk of rows' column sums of g. z NULL: g = dy; g NULL: the
-// sums alone. A workgroup takes 64 columns and `rows` rows, four rows at a time.
-template <typename S>
+// sums alone. A lane takes eight columns, cg lanes (a power of two) a row, 256 / cg rows at a time; the block's sums
+// of a column are added in a fixed order through LDS.
+template <typename S, bool VEC>
 __global__ void __launch_bounds__(256) linear_slope_kernel(const S* __restrict__ dy, long long ld, const S* __restrict__ z,
-                                                           int act, int M, int N, int Np, int rows, S* __restrict__ g,
-                                                           float* __restrict__ part) {
-  __shared__ float sum[4][64];
-  const int l = threadIdx.x & 63, w = threadIdx.x >> 6, n = blockIdx.x * 64 + l;
-  const int r0 = blockIdx.y * rows, r1 = min(M, r0 + rows);
-  float s = 0.f;
+                                                           int act, int M, int N, int Np, int cg, int rows,
+                                                           S* __restrict__ g, float* __restrict__ part) {
+  __shared__ float sum[256][9];
+  const int c = threadIdx.x % cg, n = (blockIdx.x * cg + c) * 8, step = 256 / cg;
+  const long long r0 = (long long)blockIdx.y * rows;
+  const int r1 = (int)min((long long)M - r0, (long long)rows);
+  float s[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) s[j] = 0.f;
   if (n < Np)
-#pragma unroll 4
-    for (int r = r0 + w; r < r1; r += 4) {
-      float v = 0.f;
-      if (n < N) {
-        v = (float)dy[r * ld + n];
-        if (z) v *= slope_of(act, (float)z[(long long)r * N + n]);
+#pragma unroll 2
+    for (int r = threadIdx.x / cg; r < r1; r += step) {
+      const long long m = r0 + r;
+      float v[8], t[8];
+      if constexpr (VEC) {
+        load_pack<S, 8>(dy + m * ld + n, v);
+      } else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = n + j < N ? (float)dy[m * ld + n + j] : 0.f;
       }
-      if (g) g[(long long)r * Np + n] = (S)v;
-      s += v;
+      if (z) {
+        load_pack<S, 8>(z + m * Np + n, t);
+        slope_of<sizeof(S) == 2, 8>(act, t, v);
+        if constexpr (!VEC)   // z's rows are not filled behind N
+#pragma unroll
+          for (int j = 0; j < 8; ++j) v[j] = n + j < N ? v[j] : 0.f;
+      }
+      if (g) store_pack<S, 8>(g + m * Np + n, v);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) s[j] += v[j];
     }
   if (!part) return;
-  sum[w][l] = s;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) sum[threadIdx.x][j] = s[j];
   __syncthreads();
-  if (w == 0 && n < N) part[(long long)blockIdx.y * N + n] = (sum[0][l] + sum[1][l]) + (sum[2][l] + sum[3][l]);
+  for (int i = threadIdx.x; i < cg * 8; i += 256) {
+    const int at = blockIdx.x * cg * 8 + i;
+    if (at >= N) continue;
+    float v = 0.f;
+    for (int k = 0; k < step; ++k) v += sum[k * cg + i / 8][i & 7];
+    part[(long long)blockIdx.y * N + at] = v;
+  }
 }
 
 template <typename S>
@@ -483,6 +660,36 @@ struct Mat {            // an operand as the kernel reads it
 
 inline int up8(int n) { return (n + 7) / 8 * 8; }
 inline unsigned blocks_for(long long n) { return (unsigned)std::min<long long>((n + 255) / 256, 8192); }
+
+// Tile and split of a product by what a round of workgroups costs, measured on 16384 x 8192 outputs over 2 to 128 steps of 64 k:
+// 256 x 256 tiles, one workgroup a CU, 20 us + 1.6 us a step; 128 x 128, two a CU, 6 us + 1.0 us a step. So large
+// tiles for long sums over many tiles (8192^3: 0.85 ms against 1.06), small ones for short sums and where their rounds fit
+// better (25792 x 2048 over 512: 88 us against 126). A split writes and reads its slabs at 4 bytes a sum.
+struct Shape {
+  int tile, per;
+  long long tiles;
+};
+inline Shape shape_of(int M, int N, int steps, int size) {
+  Shape best{};
+  double least = 1e300;
+  for (int t : {128, 256}) {
+    const long long tiles = (long long)((M + t - 1) / t) * ((N + t - 1) / t);
+    const double fixed = t == 256 ? 20 : 6, each = t == 256 ? 1.6 : 1.0, slots = t == 256 ? 256 : 512;
+    for (int p = 1; p <= 64; p = p < 8 ? p + 1 : p + p / 4) {
+      const int per = ((steps + p - 1) / p + 1) / 2 * 2;   // the kernel takes steps in pairs
+      const int splits = (steps + per - 1) / per;
+      if (p > 1 && (per < 4 || splits < 2)) break;
+      const double rounds = std::ceil((double)tiles * splits / slots);
+      double us = rounds * (fixed + each * per);
+      if (splits > 1) us += 4 + (double)M * N * (8.0 * splits + size) * 0.25e-6;
+      if (us < least) {
+        least = us;
+        best = Shape{t, per, tiles};
+      }
+    }
+  }
+  return best;
+}
 
 // A pass of the product: lays its operands out, multiplies, joins. `run` false: takes the workspace, launches nothing.
 struct Pass {
@@ -545,7 +752,6 @@ struct Pass {
 
   template <typename H, typename S, bool AKC, bool BKC>
   void product(const Mat& A, const Mat& B, int M, int N, int K, const Epi& e) {
-    constexpr int BM = 128, BN = 128;
     GemmArgs a{};
     a.M = M; a.N = N; a.K = K;
     a.lda = A.ld; a.ldb = B.ld; a.a_bytes = A.bytes; a.b_bytes = B.bytes;
@@ -553,22 +759,33 @@ struct Pass {
     a.e = e;
     a.e.ea = A.ex; a.e.eb = B.ex;
     a.ksteps = (K + kBK - 1) / kBK;
-    const int terms = __is_same(S, float) ? 3 : 1;
-    const long long tiles = (long long)((M + BM - 1) / BM) * ((N + BN - 1) / BN), steps = (long long)terms * a.ksteps;
-    if (tiles > 0x7fffffffLL || steps > 0x7fffffffLL || A.ld > (1 << 21) || B.ld > (1 << 21)) { rc = SE_E_UNSUPPORTED; return; }
+    const long long steps = (long long)(__is_same(S, float) ? 3 : 1) * a.ksteps;
+    if (steps > 0x3fffffffLL || A.ld > (1 << 21) || B.ld > (1 << 21)) { rc = SE_E_UNSUPPORTED; return; }
     a.steps = (int)steps;
-    // two workgroups share a CU: split the reduction until 512 run, eight tiles of it at least to a split
-    int splits = 1;
-    if (tiles < 384) splits = (int)std::max<long long>(1, std::min<long long>(512 / tiles, steps / 8));
-    a.per = (a.steps + splits - 1) / splits;
+    const Shape c = shape_of(M, N, a.steps, sizeof(S));
+    if (c.tiles > 0x7fffffffLL) { rc = SE_E_UNSUPPORTED; return; }
+    a.per = c.per;
     a.splits = (a.steps + a.per - 1) / a.per;
     if (a.splits > 1) a.slab = ws.take<float>((long long)a.splits * M * N);
     if (!run || rc != SE_OK) return;
-    hipLaunchKernelGGL((linear_gemm_kernel<H, S, AKC, BKC, BM, BN, 2, 2>), dim3((unsigned)tiles, a.splits), dim3(256), 0,
-                       st, a);
+    const unsigned tiles = (unsigned)c.tiles;
+    if (c.tile == 256)
+      hipLaunchKernelGGL((linear_gemm_kernel<H, S, AKC, BKC, 256, 256, 2, 2>), dim3(tiles, a.splits), dim3(256), 0,
+                         st, a);
+    else
+      hipLaunchKernelGGL((linear_gemm_kernel<H, S, AKC, BKC, 128, 128, 2, 2>), dim3(tiles, a.splits), dim3(256), 0,
+                         st, a);
     launched();
     if (a.splits > 1) {
-      hipLaunchKernelGGL(linear_join_kernel<S>, dim3(blocks_for((long long)M * ((N + 3) / 4))), dim3(256), 0, st, a);
+      // 8 columns a thread where the rows of everything are aligned for it
+      auto ok = [&](int v) {
+        const uintptr_t al = std::min<int>(16, v * sizeof(S)) - 1;
+        return N % v == 0 && (((uintptr_t)e.C | (uintptr_t)e.bias | (uintptr_t)e.res) & al) == 0 && e.ldc % v == 0 &&
+               (!e.res || e.ldr % v == 0);
+      };
+      const long long mn = (long long)M * N;
+      if (ok(4)) hipLaunchKernelGGL((linear_join_kernel<S, 4>), dim3(blocks_for(mn / 4)), dim3(256), 0, st, a);
+      else hipLaunchKernelGGL((linear_join_kernel<S, 1>), dim3(blocks_for(mn)), dim3(256), 0, st, a);
       launched();
     }
   }
@@ -585,7 +802,7 @@ int forward(const se_linear_desc* d, const void* x, const void* w, const void* b
   const Mat A = f32 ? p.planes(x, d->ldx, d->M, d->K, true) : p.half(x, d->ldx, d->M, d->K);
   const Mat B = f32 ? p.planes(w, d->ldw, d->N, d->K, true) : p.half(w, d->ldw, d->N, d->K);
   Epi e{};
-  e.C = y; e.z = z; e.bias = bias; e.res = res; e.ldc = d->N; e.ldr = d->ldr; e.act = d->act;
+  e.C = y; e.z = z; e.bias = bias; e.res = res; e.ldc = d->N; e.ldr = d->ldr; e.ldz = up8(d->N); e.act = d->act;
   p.template product<H, S, true, true>(A, B, d->M, d->N, d->K, e);
   return p.rc;
 }
@@ -599,14 +816,25 @@ int backward(const se_linear_desc* d, const void* dy, const void* x, const void*
   const bool sloped = d->act != SE_LINACT_NONE, prod = dx || dw;
   // g: dy itself where nothing multiplies it and the product can read it as it lies
   const bool as_is = !sloped && (f32 || (d->ldr % 8 == 0 && N % 8 == 0 && ((uintptr_t)dy & 15) == 0));
-  const int Np = f32 ? N : up8(N);
+  const int Np = up8(N);
   S* g = prod && !as_is ? p.ws.template take<S>((long long)M * Np) : nullptr;
-  const int rows = std::max(64, (int)(((long long)M + 127) / 128)), parts = (M + rows - 1) / rows;
+  int cg = 1;
+  while (cg < 64 && cg * 8 < Np) cg *= 2;
+  // chunks of rows: about 2048 workgroups, each of at least four turns
+  const int across = (Np + cg * 8 - 1) / (cg * 8), turn = 256 / cg;
+  const long long chunks = std::max(1, std::min(512, 2048 / across));
+  const int rows = (int)std::max<long long>(4 * turn, (M + chunks - 1) / chunks), parts = (M + rows - 1) / rows;
   float* part = db ? p.ws.template take<float>((long long)parts * N) : nullptr;
   if (p.run && (part || g)) {
-    hipLaunchKernelGGL(linear_slope_kernel<S>, dim3((Np + 63) / 64, parts), dim3(256), 0, p.st,
-                       static_cast<const S*>(dy), d->ldr, sloped ? static_cast<const S*>(z) : nullptr, d->act, M, N, Np,
-                       rows, g, part);
+    const bool vec = N % 8 == 0 && ((uintptr_t)dy & 15) == 0 && d->ldr % (16 / sizeof(S)) == 0;
+    const S* zs = sloped ? static_cast<const S*>(z) : nullptr;
+    const S* dys = static_cast<const S*>(dy);
+    if (vec)
+      hipLaunchKernelGGL((linear_slope_kernel<S, true>), dim3(across, parts), dim3(256), 0, p.st, dys, d->ldr, zs, d->act,
+                         M, N, Np, cg, rows, g, part);
+    else
+      hipLaunchKernelGGL((linear_slope_kernel<S, false>), dim3(across, parts), dim3(256), 0, p.st, dys, d->ldr, zs, d->act,
+                         M, N, Np, cg, rows, g, part);
     p.launched();
     if (part) {
       hipLaunchKernelGGL(linear_bias_kernel<S>, dim3((N + 63) / 64), dim3(1024), 0, p.st, part, parts, N,
@@ -673,7 +901,7 @@ extern "C" int se_linear_fwd(const se_linear_desc* d, const void* x, const void*
                              void* y, void* z, void* ws, size_t ws_bytes, void* stream) {
   const int rc = check(d);
   if (rc != SE_OK) return rc;
-  if (!x || !w || !y) return SE_E_ARG;
+  if (!x || !w || !y || ((uintptr_t)z & 15) || ((uintptr_t)ws & 15)) return SE_E_ARG;
   const size_t need = se_linear_fwd_workspace_size(d, x, w);
   if (need && (!ws || ws_bytes < need)) return SE_E_WORKSPACE;
   Pass p{Carve{static_cast<char*>(ws)}, true, se::as_stream(stream)};
@@ -694,7 +922,7 @@ extern "C" int se_linear_bwd(const se_linear_desc* d, const void* dy, const void
   const int rc = check(d);
   if (rc != SE_OK) return rc;
   if (!dy || (dx && !w) || (dw && !x) || (!dx && !dw && !db) || (d->act != SE_LINACT_NONE && !z)) return SE_E_ARG;
-  if (d->M > 1 && d->ldr < d->N) return SE_E_ARG;
+  if ((d->M > 1 && d->ldr < d->N) || ((uintptr_t)z & 15) || ((uintptr_t)ws & 15)) return SE_E_ARG;
   const size_t need = se_linear_bwd_workspace_size(d, dy, x, w, dx != nullptr, dw != nullptr, db != nullptr);
   if (need && (!ws || ws_bytes < need)) return SE_E_WORKSPACE;
   Pass p{Carve{static_cast<char*>(ws)}, true, se::as_stream(stream)};

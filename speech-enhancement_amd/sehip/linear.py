@@ -195,11 +195,11 @@ def _act_code(act) -> int:
 
 
 def _act_forward(x, w, b, res, act, keep):
-    """(y, x as the kernel read it, z); z [M, N] only where `keep` and the activation needs it."""
+    """(y, x as the kernel read it, z); z (rows of a multiple of 8) only where `keep` and the activation needs it."""
     n, k = w.shape
     m = x.numel() // k
     y = torch.empty(x.shape[:-1] + (n,), device=x.device, dtype=x.dtype)
-    z = torch.empty((m, n), device=x.device, dtype=x.dtype) if keep and act != ACT_NONE else None
+    z = torch.empty((m, (n + 7) // 8 * 8), device=x.device, dtype=x.dtype) if keep and act != ACT_NONE else None
     x2, ldx = glue.as_rows(x, k)
     if m:
         w2, ldw = glue.as_rows(w, k)
