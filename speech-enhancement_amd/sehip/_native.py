@@ -8,7 +8,6 @@ torch are then valid inside the library.
 """
 from __future__ import annotations
 
-import contextlib
 import ctypes
 import os
 import re
@@ -243,12 +242,28 @@ def stream_of(t: torch.Tensor) -> int:
     return torch.cuda.current_stream(t.device).cuda_stream
 
 
-def on_device_of(t: torch.Tensor):
-    """Context in which launches go to t's device (nothing to do where it is the current one)."""
-    return _NOTHING if t.device.index == torch.cuda.current_device() else torch.cuda.device(t.device)
+def launch(index: int, what: str, fn, *args) -> None:
+    """fn(*args, stream) with GPU `index` current, stream its current one; RuntimeError unless it returns SE_OK."""
+    if _get_device() == index:
+        rc = fn(*args, _raw_stream(index))
+    else:
+        with torch.cuda.device(index):
+            rc = fn(*args, _raw_stream(index))
+    if rc:
+        check(rc, what)
 
 
-_NOTHING = contextlib.nullcontext()
+def _get_device() -> int:
+    return torch.cuda.current_device()
+
+
+def _raw_stream(index: int) -> int:
+    return torch.cuda.current_stream(index).cuda_stream
+
+
+# the same two answers without the objects around them, where this torch has them (a launch's host time)
+_get_device = getattr(torch._C, "_cuda_getDevice", _get_device)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", _raw_stream)
 
 
 def ptr(t) -> int | None:

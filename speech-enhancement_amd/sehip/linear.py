@@ -178,6 +178,7 @@ def linear(x, module: torch.nn.Linear, feature_major_out=False):
     return linear_halves(x, [module.weight], [module.bias], feature_major_out)
 
 
+_FEW_ROWS = 0   # up to so many rows se_linear_fwd takes no workspace
 ACT_NONE, ACT_RELU, ACT_GELU, ACT_GELU_TANH, ACT_SILU = range(5)   # SE_LINACT_* (include/sehip.h)
 
 
@@ -195,59 +196,64 @@ def _act_code(act) -> int:
 
 
 def _act_forward(x, w, b, res, act, keep):
-    """(y, x as the kernel read it, z); z (rows of a multiple of 8) only where `keep` and the activation needs it."""
+    """(y, x as the kernel read it, its rows' distance, z); z (rows of a multiple of 8) only where `keep` and the activation
+    needs it."""
     n, k = w.shape
     m = x.numel() // k
-    y = torch.empty(x.shape[:-1] + (n,), device=x.device, dtype=x.dtype)
-    z = torch.empty((m, (n + 7) // 8 * 8), device=x.device, dtype=x.dtype) if keep and act != ACT_NONE else None
-    x2, ldx = glue.as_rows(x, k)
+    y = x.new_empty(x.shape[:-1] + (n,))
+    z = x.new_empty((m, (n + 7) // 8 * 8)) if keep and act else None
+    x2, ldx = (x, k) if x.is_contiguous() else glue.as_rows(x, k)
     if m:
-        w2, ldw = glue.as_rows(w, k)
+        w2, ldw = (w, k) if w.is_contiguous() else glue.as_rows(w, k)
         r2, ldr = (None, n) if res is None else glue.as_rows(res, n)
         lib = N.lib()
-        d = N.LinearDesc(m, n, k, act, N.DTYPES[x.dtype], ldx, ldw, ldr)
-        p = ctypes.byref(d)
+        p = ctypes.byref(N.LinearDesc(m, n, k, act, N.DTYPES[x.dtype], ldx, ldw, ldr))
         xp, wp = x2.data_ptr(), w2.data_ptr()
-        with N.on_device_of(x):
-            need = lib.se_linear_fwd_workspace_size(p, xp, wp)
-            ws = torch.empty(need, device=x.device, dtype=torch.uint8) if need else None
-            N.check(lib.se_linear_fwd(p, xp, wp, N.ptr(b), N.ptr(r2), y.data_ptr(), N.ptr(z), N.ptr(ws), need,
-                                      N.stream_of(x)), "se_linear_fwd")
-    return y, x2, z
+        # one or a few rows need no workspace: it is not asked for
+        size = 0 if m <= _FEW_ROWS else lib.se_linear_fwd_workspace_size(p, xp, wp)
+        ws = x.new_empty(size, dtype=torch.uint8) if size else None
+        N.launch(x.get_device(), "se_linear_fwd", lib.se_linear_fwd, p, xp, wp, N.ptr(b), N.ptr(r2), y.data_ptr(), N.ptr(z),
+                 N.ptr(ws), size)
+    return y, x2, ldx, z
+
+
+def _act_backward(ctx, gy):
+    x, w, z = ctx.saved_tensors
+    act, ldx = ctx.cfg
+    n, k = w.shape
+    m = x.numel() // k
+    need = ctx.needs_input_grad
+    new = x.new_empty if m else x.new_zeros
+    dx = torch.empty_like(x, memory_format=torch.contiguous_format) if need[0] else None
+    dw = new((n, k)) if need[1] else None
+    db = new(n) if need[2] else None
+    if m and (need[0] or need[1] or need[2]):
+        g2, ldg = (gy, n) if gy.is_contiguous() and gy.dtype == x.dtype else glue.as_rows(gy, n, x.dtype)
+        w2, ldw = (w, k) if w.is_contiguous() else glue.as_rows(w, k)
+        lib = N.lib()
+        p = ctypes.byref(N.LinearDesc(m, n, k, act, N.DTYPES[x.dtype], ldx, ldw, ldg))
+        gp, xp, wp = g2.data_ptr(), x.data_ptr(), w2.data_ptr()
+        size = lib.se_linear_bwd_workspace_size(p, gp, xp, wp, need[0], need[1], need[2])
+        ws = x.new_empty(size, dtype=torch.uint8) if size else None
+        N.launch(x.get_device(), "se_linear_bwd", lib.se_linear_bwd, p, gp, xp, wp, N.ptr(z), N.ptr(dx), N.ptr(dw), N.ptr(db),
+                 N.ptr(ws), size)
+    return dx, dw, db, gy if need[3] else None, None
+
+
+_act_backward_once = once_differentiable(_act_backward)
 
 
 class _LinearAct(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w, b, res, act):
-        y, x2, z = _act_forward(x, w, b, res, act, True)
+        y, x2, ldx, z = _act_forward(x, w, b, res, act, True)
         ctx.save_for_backward(x2, w, z)
-        ctx.act = act
+        ctx.cfg = (act, ldx)
         return y
 
     @staticmethod
-    @once_differentiable
-    def backward(ctx, gy):
-        x, w, z = ctx.saved_tensors
-        n, k = w.shape
-        m = x.numel() // k
-        need = ctx.needs_input_grad
-        new = torch.empty if m else torch.zeros
-        dx = torch.empty(x.shape, device=x.device, dtype=x.dtype) if need[0] else None
-        dw = new((n, k), device=x.device, dtype=x.dtype) if need[1] else None
-        db = new(n, device=x.device, dtype=x.dtype) if need[2] else None
-        if m and (need[0] or need[1] or need[2]):
-            g2, ldg = glue.as_rows(gy, n, x.dtype)
-            ldx, (w2, ldw) = glue.as_rows(x, k)[1], glue.as_rows(w, k)
-            lib = N.lib()
-            d = N.LinearDesc(m, n, k, ctx.act, N.DTYPES[x.dtype], ldx, ldw, ldg)
-            p = ctypes.byref(d)
-            gp, xp, wp = g2.data_ptr(), x.data_ptr(), w2.data_ptr()
-            with N.on_device_of(x):
-                size = lib.se_linear_bwd_workspace_size(p, gp, xp, wp, need[0], need[1], need[2])
-                ws = torch.empty(size, device=x.device, dtype=torch.uint8) if size else None
-                N.check(lib.se_linear_bwd(p, gp, xp, wp, N.ptr(z), N.ptr(dx), N.ptr(dw), N.ptr(db), N.ptr(ws), size,
-                                          N.stream_of(x)), "se_linear_bwd")
-        return dx, dw, db, gy if need[3] else None, None
+    def backward(ctx, gy):   # with create_graph, a result that refuses to be differentiated again
+        return _act_backward_once(ctx, gy) if torch.is_grad_enabled() else _act_backward(ctx, gy)
 
 
 def linear_act(x: torch.Tensor, module: nn.Linear, act: nn.Module | None = None,
@@ -259,13 +265,13 @@ def linear_act(x: torch.Tensor, module: nn.Linear, act: nn.Module | None = None,
     NaN, not always the one of the two that fp32 products would give. A second derivative is refused."""
     code = _act_code(act)
     w, b = module.weight, module.bias
-    for t in (x, w, b, residual):
-        if t is None:
-            continue
-        if not t.is_cuda or t.device != x.device:
-            raise RuntimeError("sehip linear_act: all tensors must be on one GPU (there is no CPU fallback)")
-        if t.dtype != x.dtype or t.dtype not in N.DTYPES:
-            raise RuntimeError(f"sehip linear_act: {t.dtype} beside a {x.dtype} input (one of fp32, bf16, fp16 throughout)")
+    dev, dt = x.get_device(), x.dtype
+    if dev < 0 or w.get_device() != dev or (b is not None and b.get_device() != dev) or (
+            residual is not None and residual.get_device() != dev):
+        raise RuntimeError("sehip linear_act: all tensors must be on one GPU (there is no CPU fallback)")
+    if dt not in N.DTYPES or w.dtype != dt or (b is not None and b.dtype != dt) or (
+            residual is not None and residual.dtype != dt):
+        raise RuntimeError(f"sehip linear_act: input {dt}, weight {w.dtype} (one of fp32, bf16, fp16 throughout)")
     n, k = w.shape
     if n == 0 or k == 0 or x.dim() == 0 or x.shape[-1] != k:
         raise RuntimeError(f"sehip linear_act: input {tuple(x.shape)}, weight {tuple(w.shape)}")

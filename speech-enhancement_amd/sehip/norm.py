@@ -15,12 +15,13 @@ fp16 storage with the weight and bias in the same type or in fp32, the weight's 
 bias's gradients summed in a fixed order. CPU tensors raise."""
 from __future__ import annotations
 
+import math
+
 import torch
 import torch.nn as nn
 from torch.autograd.function import once_differentiable
 
 from . import _native as N
-from . import functional as F
 from . import glue
 
 _ACT_NONE, _ACT_PRELU, _ACT_ELU = 0, 1, 2
@@ -107,54 +108,53 @@ def bn_act(norm: nn.Module, act: nn.Module, x: torch.Tensor) -> torch.Tensor:
 
 
 def _ln_forward(x, C, weight, bias, eps, keep):
-    """(y, rows of x as the kernel read them, save) of one launch; save None unless `keep`."""
-    x2, ld = glue.as_rows(x, C)
+    """(y, rows of x as the kernel read them, their distance, save) of one launch; save None unless `keep`."""
+    x2, ld = (x, C) if x.is_contiguous() else glue.as_rows(x, C)
     rows = x.numel() // C
-    y = torch.empty(x.shape, device=x.device, dtype=x.dtype)
-    save = torch.empty((2, rows), device=x.device, dtype=torch.float32) if keep else None
+    y = torch.empty_like(x, memory_format=torch.contiguous_format)
+    save = x.new_empty((2, rows), dtype=torch.float32) if keep else None
     if rows:
         wt = weight if weight is not None else bias if bias is not None else x
-        with N.on_device_of(x):
-            N.check(N.lib().se_layer_norm_fwd(x2.data_ptr(), ld, rows, C, N.ptr(weight), N.ptr(bias), eps, y.data_ptr(),
-                                              N.ptr(save), N.DTYPES[x.dtype], N.DTYPES[wt.dtype], N.stream_of(x)),
-                    "se_layer_norm_fwd")
-    return y, x2, save
+        N.launch(x.get_device(), "se_layer_norm_fwd", N.lib().se_layer_norm_fwd, x2.data_ptr(), ld, rows, C, N.ptr(weight),
+                 N.ptr(bias), eps, y.data_ptr(), N.ptr(save), N.DTYPES[x.dtype], N.DTYPES[wt.dtype])
+    return y, x2, ld, save
+
+
+def _ln_backward(ctx, gy):
+    x, weight, save = ctx.saved_tensors
+    C, ldx, bdt = ctx.cfg
+    need = ctx.needs_input_grad
+    rows = x.numel() // C
+    wdt = weight.dtype if weight is not None else bdt or x.dtype
+    dx = torch.empty_like(x, memory_format=torch.contiguous_format) if need[0] else None
+    new = x.new_empty if rows else x.new_zeros
+    dw = new(C, dtype=wdt) if need[1] else None
+    db = new(C, dtype=wdt) if need[2] else None
+    if rows:
+        g2, ldg = (gy, C) if gy.is_contiguous() and gy.dtype == x.dtype else glue.as_rows(gy, C, x.dtype)
+        lib = N.lib()
+        size = lib.se_layer_norm_workspace_size(rows, C) if need[1] or need[2] else 0
+        ws = x.new_empty(size, dtype=torch.uint8) if size else None
+        N.launch(x.get_device(), "se_layer_norm_bwd", lib.se_layer_norm_bwd, g2.data_ptr(), ldg, x.data_ptr(), ldx, rows, C,
+                 N.ptr(weight), save.data_ptr(), N.ptr(dx), N.ptr(dw), N.ptr(db), N.DTYPES[x.dtype], N.DTYPES[wdt], N.ptr(ws),
+                 size)
+    return dx, dw, db, None, None
+
+
+_ln_backward_once = once_differentiable(_ln_backward)
 
 
 class _LayerNorm(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, C, eps):
-        y, x2, save = _ln_forward(x, C, weight, bias, eps, True)
+        y, x2, ld, save = _ln_forward(x, C, weight, bias, eps, True)
         ctx.save_for_backward(x2, weight, save)
-        ctx.cfg = (C, None if bias is None else bias.dtype)
+        ctx.cfg = (C, ld, None if bias is None else bias.dtype)
         return y
 
     @staticmethod
-    @once_differentiable
-    def backward(ctx, gy):
-        x, weight, save = ctx.saved_tensors
-        C, bdt = ctx.cfg
-        need = ctx.needs_input_grad
-        rows = x.numel() // C
-        wdt = weight.dtype if weight is not None else bdt or x.dtype
-        dx = torch.empty(x.shape, device=x.device, dtype=x.dtype) if need[0] else None
-        new = torch.empty if rows else torch.zeros
-        dw = new(C, device=x.device, dtype=wdt) if need[1] else None
-        db = new(C, device=x.device, dtype=wdt) if need[2] else None
-        if rows:
-            g2, ldg = glue.as_rows(gy, C, x.dtype)
-            ldx = glue.as_rows(x, C)[1]
-            lib = N.lib()
-            with N.on_device_of(x):
-                ws = F._workspace(lib.se_layer_norm_workspace_size(rows, C), x.device) if need[1] or need[2] else None
-                N.check(lib.se_layer_norm_bwd(g2.data_ptr(), ldg, x.data_ptr(), ldx, rows, C, N.ptr(weight),
-                                              save.data_ptr(), N.ptr(dx), N.ptr(dw), N.ptr(db), N.DTYPES[x.dtype],
-                                              N.DTYPES[wdt], N.ptr(ws), 0 if ws is None else ws.numel(),
-                                              N.stream_of(x)), "se_layer_norm_bwd")
-        if weight is not None:
-            dw = None if dw is None else dw.view(weight.shape)
-            db = None if db is None else db.view(weight.shape)
-        return dx, dw, db, None, None
+    def backward(ctx, gy):   # with create_graph, a result that refuses to be differentiated again
+        return _ln_backward_once(ctx, gy) if torch.is_grad_enabled() else _ln_backward(ctx, gy)
 
 
 def layer_norm(norm: nn.LayerNorm, x: torch.Tensor) -> torch.Tensor:
@@ -163,27 +163,30 @@ def layer_norm(norm: nn.LayerNorm, x: torch.Tensor) -> torch.Tensor:
     derivative is refused."""
     shape, w, b = norm.normalized_shape, norm.weight, norm.bias
     k = len(shape)
-    if tuple(x.shape[x.dim() - k:]) != tuple(shape) or x.dim() < k:
+    if x.shape[-k:] != shape:
         raise RuntimeError(f"sehip layer_norm: input {tuple(x.shape)} does not end in {tuple(shape)}")
-    for t in (x, w, b):
-        if t is not None and (not t.is_cuda or t.device != x.device):
-            raise RuntimeError("sehip layer_norm: x, weight and bias must be on one GPU (there is no CPU fallback)")
-    if x.dtype not in N.DTYPES:
-        raise RuntimeError(f"sehip layer_norm: unsupported storage type {x.dtype} (fp32, bf16, fp16)")
-    wdt = {t.dtype for t in (w, b) if t is not None}
-    if len(wdt) > 1 or not wdt <= {x.dtype, torch.float32}:
-        raise RuntimeError(f"sehip layer_norm: weight and bias {sorted(map(str, wdt))} beside a {x.dtype} input (both in "
-                           "its type or both in fp32)")
-    C = 1
-    for n in shape:
-        C *= n
+    dev, dt = x.get_device(), x.dtype
+    if dev < 0 or (w is not None and w.get_device() != dev) or (b is not None and b.get_device() != dev):
+        raise RuntimeError("sehip layer_norm: x, weight and bias must be on one GPU (there is no CPU fallback)")
+    if dt not in N.DTYPES:
+        raise RuntimeError(f"sehip layer_norm: unsupported storage type {dt} (fp32, bf16, fp16)")
+    wdt = dt if w is None and b is None else w.dtype if w is not None else b.dtype
+    if (wdt != dt and wdt != torch.float32) or (b is not None and b.dtype != wdt):
+        raise RuntimeError(f"sehip layer_norm: weight and bias {wdt}, {None if b is None else b.dtype} beside a {dt} input (both "
+                           "in its type or both in fp32)")
+    if not ((w is None or w.is_contiguous()) and (b is None or b.is_contiguous())):
+        raise RuntimeError("sehip layer_norm: weight and bias must be contiguous")
+    if k == 1:
+        C = shape[0]
+        if C == 0:
+            raise RuntimeError("sehip layer_norm: normalised over no elements")
+        return _layer_norm(x, w, b, C, norm.eps)
+    C = math.prod(shape)
     if C == 0:
         raise RuntimeError("sehip layer_norm: normalised over no elements")
-    if k > 1:
-        if not all(t is None or t.is_contiguous() for t in (w, b)):
-            raise RuntimeError("sehip layer_norm: weight and bias must be contiguous")
-        return _layer_norm(x.flatten(x.dim() - k), w, b, C, float(norm.eps)).view(x.shape)
-    return _layer_norm(x, w, b, C, float(norm.eps))
+    # the normalised axes as one (views of w and b, so that their gradients come back in their own shapes)
+    return _layer_norm(x.flatten(x.dim() - k), w if w is None else w.view(C), b if b is None else b.view(C), C,
+                       norm.eps).view(x.shape)
 
 
 def _layer_norm(x, w, b, C, eps):

@@ -20,6 +20,8 @@ There is no CPU path.
 from __future__ import annotations
 
 
+import operator
+
 import numpy as np
 import torch
 
@@ -198,6 +200,7 @@ class AdamW(torch.optim.Optimizer):
                 st["step"] += 1
 
 
+_dtype_of = operator.attrgetter("dtype")
 SCALE_BLOCK = 128   # SE_ADAMW_BLOCK (include/sehip.h)
 _STATE_KEYS = {32: ("exp_avg", "exp_avg_sq"),
                8: ("exp_avg", "exp_avg_scale", "exp_avg_root", "exp_avg_root_scale")}
@@ -234,23 +237,22 @@ def _multi(params, columns, types, bits, step, lr, betas, eps, weight_decay, see
     dev, dt = p0.device, p0.dtype
     if dev.type != "cuda" or dt not in N.DTYPES:
         raise RuntimeError("sehip adamw: parameters must be fp32, bf16 or fp16 CUDA tensors (there is no CPU path)")
-    sizes = [p.numel() for p in params]
+    T = torch.Tensor
+    index = p0.get_device()
+    sizes = list(map(T.numel, params))
     blocks = [-(-k // SCALE_BLOCK) for k in sizes] if bits == 8 else None
     arr = np.zeros(n, dtype=_TENSOR)
     for name, ts, ty in zip(_TENSOR.names, (params, *columns), (dt, *types)):
         want = blocks if name.endswith("scale") else sizes
-        for t, k in zip(ts, want):
-            if t.dtype != ty or t.numel() != k or not t.is_contiguous() or t.device != dev:
-                raise RuntimeError(f"sehip adamw: {name} of {t.numel()} {t.dtype} on {t.device}, expected {k} contiguous {ty} "
-                                   f"on {dev}")
-        arr[name] = [t.data_ptr() for t in ts]
+        if (list(map(T.numel, ts)) != want or set(map(_dtype_of, ts)) != {ty} or set(map(T.get_device, ts)) != {index}
+                or not all(map(T.is_contiguous, ts))):
+            raise RuntimeError(f"sehip adamw: {name}: not all contiguous {ty} tensors of the parameters' sizes on {dev}")
+        arr[name] = list(map(T.data_ptr, ts))
     arr["numel"] = sizes
     if torch.cuda.is_current_stream_capturing():
         raise RuntimeError("sehip adamw: a captured graph would repeat this step's count and bias corrections")
-    with N.on_device_of(p0):
-        N.check(N.lib().se_adamw_multi(arr.ctypes.data, n, N.DTYPES[dt], bits, float(lr), float(betas[0]), float(betas[1]),
-                                       float(eps), float(weight_decay), int(step), int(seed) & 0xFFFFFFFFFFFFFFFF,
-                                       N.stream_of(p0)), "se_adamw_multi")
+    N.launch(index, "se_adamw_multi", N.lib().se_adamw_multi, arr.ctypes.data, n, N.DTYPES[dt], bits, float(lr), float(betas[0]),
+             float(betas[1]), float(eps), float(weight_decay), int(step), int(seed) & 0xFFFFFFFFFFFFFFFF)
     written = [*params, *columns[1], *columns[2]]
     torch.autograd.graph.increment_version(written)
 
