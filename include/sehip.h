@@ -804,7 +804,8 @@ int se_layer_norm_bwd(const void* dy, long long dy_stride, const void* x, long l
  * backward, rows ceil(N / 8) * 8 apart, on 16 bytes. All of one storage type; fp32 accumulation, y rounded once.
  * Backward: g = dy act'(z) (dy's rows ldr apart), dx = g W, dw = g^T x,
  * db = sum_m g; what is not NULL is written, z is needed where act is not
- * SE_LINACT_NONE. The workspace sizes depend on the pointers' alignment.
+ * SE_LINACT_NONE. The workspace sizes depend on the pointers' alignment; the
+ * forward of up to SE_LINEAR_FEW_ROWS rows takes none.
  * ------------------------------------------------------------------------ */
 enum {
   SE_LINACT_NONE = 0,
@@ -813,6 +814,7 @@ enum {
   SE_LINACT_GELU_TANH = 3,  /* the tanh form                                    */
   SE_LINACT_SILU = 4
 };
+#define SE_LINEAR_FEW_ROWS 64
 typedef struct se_linear_desc {
   int M, N, K;
   int act, dtype;

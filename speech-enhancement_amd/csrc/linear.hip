@@ -496,6 +496,87 @@ __global__ void __launch_bounds__(256) linear_join_kernel(const GemmArgs a) {
   }
 }
 
+// ------------------------------------------------------------------ few rows
+// Up to 64 rows of x: bound by the one read of W. A workgroup takes 16 rows of W (columns of y), its waves a slice of K each;
+// a lane fetches 16 bytes of its row of W and of its rows of x straight into the fragments of v_mfma_f32_16x16x32 (fp32: four
+// v_mfma_f32_16x16x4_f32, exact products, lane group g and element j standing for k = 16 s + 4 g + j in both operands), and the
+// slices are added in order through LDS: one launch, no workspace.
+template <typename S> struct Frag { typedef f32x4 T; };
+template <> struct Frag<__bf16> { typedef bf16x8 T; };
+template <> struct Frag<_Float16> { typedef f16x8 T; };
+
+template <typename S>
+__device__ __forceinline__ f32x4 mfma16(typename Frag<S>::T a, typename Frag<S>::T b, f32x4 c) {
+  if constexpr (__is_same(S, __bf16)) return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+  else if constexpr (__is_same(S, _Float16)) return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+  else {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[j], b[j], c, 0, 0, 0);
+    return c;
+  }
+}
+
+// the 16 bytes of a row from k on; zeros behind K
+template <typename S, bool VEC>
+__device__ __forceinline__ typename Frag<S>::T few_load(const S* row, int k, int K) {
+  constexpr int E = 16 / sizeof(S);
+  typename Frag<S>::T v = {};
+  if constexpr (VEC) {
+    if (k < K) v = *reinterpret_cast<const typename Frag<S>::T*>(row + k);
+  } else {
+#pragma unroll
+    for (int j = 0; j < E; ++j)
+      if (k + j < K) v[j] = row[k + j];
+  }
+  return v;
+}
+
+template <typename S, bool VEC, int MT>
+__global__ void __launch_bounds__(1024) linear_few_kernel(const S* __restrict__ x, long long ldx, const S* __restrict__ w,
+                                                          long long ldw, int M, int N, int K, Epi e) {
+  constexpr int E = 16 / sizeof(S), KS = 4 * E, U = MT == 1 ? 8 : 4;
+  extern __shared__ float part[];   // [waves][MT][16 m][16 n]
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
+  const int r = lane & 15, g = lane >> 4, n0 = blockIdx.x * 16;
+  const int steps = (K + KS - 1) / KS, per = (steps + waves - 1) / waves;
+  const int s0 = wave * per, s1 = min(steps, s0 + per);
+  // rows behind the end repeat the last one: their products are not used
+  const S* wr = w + min(n0 + r, N - 1) * ldw;
+  const S* xr[MT];
+#pragma unroll
+  for (int t = 0; t < MT; ++t) xr[t] = x + min(16 * t + r, M - 1) * ldx;
+  f32x4 acc[MT];
+#pragma unroll
+  for (int t = 0; t < MT; ++t) acc[t] = (f32x4){0.f, 0.f, 0.f, 0.f};
+  for (int s = s0; s < s1; s += U) {
+    typename Frag<S>::T fw[U], fx[U][MT];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int k = s + u < s1 ? (s + u) * KS + g * E : K;
+      fw[u] = few_load<S, VEC>(wr, k, K);
+#pragma unroll
+      for (int t = 0; t < MT; ++t) fx[u][t] = few_load<S, VEC>(xr[t], k, K);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int t = 0; t < MT; ++t) acc[t] = mfma16<S>(fw[u], fx[u][t], acc[t]);
+  }
+#pragma unroll
+  for (int t = 0; t < MT; ++t) *reinterpret_cast<f32x4*>(part + ((wave * MT + t) * 16 + r) * 16 + 4 * g) = acc[t];
+  __syncthreads();
+  for (int i = threadIdx.x; i < MT * 256; i += blockDim.x) {
+    const int m = i >> 4, n = n0 + (i & 15);
+    if (m >= M || n >= N) continue;
+    float v[1] = {0.f}, res[1] = {0.f};
+    for (int k = 0; k < waves; ++k) v[0] += part[k * MT * 256 + i];
+    Cols<S, 1> cols;
+    cols.load(e, n);
+    if (e.res) res[0] = (float)static_cast<const S*>(e.res)[m * e.ldr + n];
+    epilogue<S, 1>(e, cols, m, n, v, res, 0);
+  }
+}
+
 // ------------------------------------------------------------------ operands laid out
 // [R][C] at ld -> rows of Cp = C rounded up to 8, zeros behind C (a matrix whose rows do not start on 16 bytes)
 __global__ void __launch_bounds__(256) linear_pack_kernel(const u16* __restrict__ x, long long ld, int R, int C, int Cp,
@@ -791,6 +872,20 @@ struct Pass {
   }
 };
 
+constexpr int kFewRows = SE_LINEAR_FEW_ROWS;
+
+template <typename S, int MT>
+void launch_few(const S* x, long long ldx, const S* w, long long ldw, int M, int N, int K, const Epi& e, bool vec,
+                hipStream_t st) {
+  const int ks = 64 / sizeof(S), most = MT == 4 ? 8 : 16;
+  int waves = 1;
+  while (waves < most && waves * 8 * ks < K) waves *= 2;   // eight fetches of 16 bytes a lane are under way at once
+  const dim3 grid((N + 15) / 16), block(waves * 64);
+  const size_t lds = (size_t)waves * MT * 256 * sizeof(float);
+  if (vec) hipLaunchKernelGGL((linear_few_kernel<S, true, MT>), grid, block, lds, st, x, ldx, w, ldw, M, N, K, e);
+  else hipLaunchKernelGGL((linear_few_kernel<S, false, MT>), grid, block, lds, st, x, ldx, w, ldw, M, N, K, e);
+}
+
 template <typename S> struct Product { using H = S; };
 template <> struct Product<float> { using H = _Float16; };
 
@@ -799,10 +894,22 @@ int forward(const se_linear_desc* d, const void* x, const void* w, const void* b
             Pass& p) {
   using H = typename Product<S>::H;
   constexpr bool f32 = __is_same(S, float);
-  const Mat A = f32 ? p.planes(x, d->ldx, d->M, d->K, true) : p.half(x, d->ldx, d->M, d->K);
-  const Mat B = f32 ? p.planes(w, d->ldw, d->N, d->K, true) : p.half(w, d->ldw, d->N, d->K);
   Epi e{};
   e.C = y; e.z = z; e.bias = bias; e.res = res; e.ldc = d->N; e.ldr = d->ldr; e.ldz = up8(d->N); e.act = d->act;
+  if (d->M <= kFewRows) {
+    if (!p.run) return p.rc;
+    const int v = 16 / sizeof(S);
+    const bool vec = d->K % v == 0 && d->ldx % v == 0 && d->ldw % v == 0 && (((uintptr_t)x | (uintptr_t)w) & 15) == 0;
+    const S* xs = static_cast<const S*>(x);
+    const S* ws = static_cast<const S*>(w);
+    if (d->M <= 16) launch_few<S, 1>(xs, d->ldx, ws, d->ldw, d->M, d->N, d->K, e, vec, p.st);
+    else if (d->M <= 32) launch_few<S, 2>(xs, d->ldx, ws, d->ldw, d->M, d->N, d->K, e, vec, p.st);
+    else launch_few<S, 4>(xs, d->ldx, ws, d->ldw, d->M, d->N, d->K, e, vec, p.st);
+    p.launched();
+    return p.rc;
+  }
+  const Mat A = f32 ? p.planes(x, d->ldx, d->M, d->K, true) : p.half(x, d->ldx, d->M, d->K);
+  const Mat B = f32 ? p.planes(w, d->ldw, d->N, d->K, true) : p.half(w, d->ldw, d->N, d->K);
   p.template product<H, S, true, true>(A, B, d->M, d->N, d->K, e);
   return p.rc;
 }

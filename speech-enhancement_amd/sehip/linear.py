@@ -178,7 +178,7 @@ def linear(x, module: torch.nn.Linear, feature_major_out=False):
     return linear_halves(x, [module.weight], [module.bias], feature_major_out)
 
 
-_FEW_ROWS = 0   # up to so many rows se_linear_fwd takes no workspace
+_FEW_ROWS = 64   # SE_LINEAR_FEW_ROWS (include/sehip.h): up to so many rows the forward takes no workspace
 ACT_NONE, ACT_RELU, ACT_GELU, ACT_GELU_TANH, ACT_SILU = range(5)   # SE_LINACT_* (include/sehip.h)
 
 

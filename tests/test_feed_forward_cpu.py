@@ -62,15 +62,18 @@ def test_linear_c_arguments():
     assert fwd(D(3, 4, 8, 0, 1, 4, 8, 4)) == -1        # rows of x would overlap
     assert fwd(D(3, 4, 8, 0, 1, 8, 4, 4)) == -1        # rows of W would
     assert fwd(D(3, 4, 1 << 22, 0, 1, 1 << 22, 1 << 22, 4)) == -3
-    d = D(3, 4, 8, 0, 0, 8, 8, 4)
+    d = D(70, 4, 8, 0, 0, 8, 8, 4)
     need = lib.se_linear_fwd_workspace_size(ctypes.byref(d), p, p)
     assert need > 0                                     # fp32: the planes
     assert fwd(d, need - 1) == -5
     assert lib.se_linear_fwd_workspace_size(ctypes.byref(D(0, 4, 8, 0, 0, 8, 8, 4)), p, p) == 0
     # bf16 on 16 bytes reads x and W as they lie; a row off 16 bytes is packed
-    assert lib.se_linear_fwd_workspace_size(ctypes.byref(D(3, 4, 8, 0, 1, 8, 8, 4)), p, p) == 0
-    assert lib.se_linear_fwd_workspace_size(ctypes.byref(D(3, 4, 7, 0, 1, 7, 7, 4)), p, p) > 0
-    d = D(3, 4, 8, 2, 1, 8, 8, 4)
+    assert lib.se_linear_fwd_workspace_size(ctypes.byref(D(70, 4, 8, 0, 1, 8, 8, 4)), p, p) == 0
+    assert lib.se_linear_fwd_workspace_size(ctypes.byref(D(70, 4, 7, 0, 1, 7, 7, 4)), p, p) > 0
+    # few rows never need one
+    for dt in range(3):
+        assert lib.se_linear_fwd_workspace_size(ctypes.byref(D(64, 4, 7, 0, dt, 7, 7, 4)), p, p) == 0
+    d = D(70, 4, 8, 2, 1, 8, 8, 4)
     bwd = lib.se_linear_bwd
     assert bwd(ctypes.byref(d), p, p, p, None, p, None, None, None, 0, None) == -1   # the slope needs z
     assert bwd(ctypes.byref(d), p, p, p, p, None, None, None, None, 0, None) == -1   # nothing wanted
