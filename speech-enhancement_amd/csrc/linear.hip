@@ -174,17 +174,17 @@ struct Cols {
 };
 
 // those columns of row m, out of the sums; res: the residual's values. Every row is aligned for V.
-template <typename S, int V>
+template <typename S, int V, bool RES>
 __device__ __forceinline__ void epilogue(const Epi& e, const Cols<S, V>& cols, long long m, int n, float (&v)[V],
                                          const float (&res)[V], int ea) {
-  if (e.ea)
+  if constexpr (sizeof(S) == 4)   // fp32: the planes' powers of two (0 where there are none)
 #pragma unroll
     for (int j = 0; j < V; ++j) v[j] = __builtin_ldexpf(v[j], ea + cols.eb[j]);
 #pragma unroll
   for (int j = 0; j < V; ++j) v[j] += cols.bias[j];
   if (e.z) store_pack<S, V>(static_cast<S*>(e.z) + m * e.ldz + n, v);
   act_of<sizeof(S) == 2, V>(e.act, v);
-  if (e.res)
+  if constexpr (RES)
 #pragma unroll
     for (int j = 0; j < V; ++j) v[j] += res[j];
   store_pack<S, V>(static_cast<S*>(e.C) + m * e.ldc + n, v);
@@ -272,46 +272,80 @@ __device__ __forceinline__ void tile_of(int id, int MT, int NT, int& mt, int& nt
   nt = in / deep;
 }
 
-// 32 rows of TN sums from `turn` through the epilogue (or into the slab), V columns a lane: the rows' residuals of four
-// turns are asked for together
-template <typename S, int V, int TN, int PITCH>
-__device__ __forceinline__ void drain(const GemmArgs& a, float* slab, const float* turn, int lane, int mb, int nb) {
-  constexpr int kWide = TN < 64 * V ? TN : 64 * V, kLanes = kWide / V, kRows = 64 / kLanes, kU = 32 / kRows < 4 ? 32 / kRows : 4;
+// 32 rows of TN sums from `turn` through the epilogue (or into the slab), V columns a lane. Stores and loads complete in the
+// order they were asked for, so nothing in the loop may wait for a load behind a store: what the columns need is
+// there before it (`arrived`), a row's power of two comes from a register of another lane, and the residuals of eight
+// turns are asked for together.
+template <typename S, int V>
+__device__ __forceinline__ void arrived(const Cols<S, V>& c) {
+#pragma unroll
+  for (int j = 0; j < V; ++j) asm volatile("" ::"v"(c.bias[j]), "v"(c.eb[j]));
+}
+template <typename S, int V, bool RES, int TN, int PITCH>
+__device__ __forceinline__ void drain(const GemmArgs& a, float* slab, const float* turn, int lane, int mb, int nb, int ea32) {
+  constexpr int kWide = TN < 64 * V ? TN : 64 * V, kLanes = kWide / V, kRows = 64 / kLanes;
+  constexpr int kU = 32 / kRows < 8 ? 32 / kRows : 8;
 #pragma unroll 1
-  for (int c = (lane % kLanes) * V; c < TN; c += kWide) {
-    const int n = nb + c;
-    if (n >= a.N) continue;   // V divides N
+  for (int c0 = 0; c0 < TN; c0 += kWide) {
+    const int c = c0 + (lane % kLanes) * V, n = nb + c;
+    const bool on = n < a.N;   // V divides N
     Cols<S, V> cols;
-    if (!slab) cols.load(a.e, n);
+    cols.load(a.e, on ? n : 0);
+    arrived(cols);
 #pragma unroll 1
-    for (int r0 = lane / kLanes; r0 < 32; r0 += kU * kRows) {
-      float res[kU][V];
-      int ea[kU];
+    for (int r0 = 0; r0 < 32; r0 += kU * kRows) {
+      float v[kU * V], res[RES ? kU * V : 1];
+      const int first = r0 + lane / kLanes;
 #pragma unroll
       for (int u = 0; u < kU; ++u) {
-        const int m = mb + r0 + u * kRows;
+        const int r = first + u * kRows;
+        float t[V];
+        load_pack<float, V>(turn + r * PITCH + c, t);
 #pragma unroll
-        for (int k = 0; k < V; ++k) res[u][k] = 0.f;
-        ea[u] = 0;
-        if (m >= a.M || slab) continue;
-        if (a.e.res) load_pack<S, V>(static_cast<const S*>(a.e.res) + m * a.e.ldr + n, res[u]);
-        if (a.e.ea) ea[u] = a.e.ea[m];
+        for (int j = 0; j < V; ++j) v[u * V + j] = t[j];
+        if constexpr (RES) {
+          const bool in = on && mb + r < a.M;
+          load_pack<S, V>(static_cast<const S*>(a.e.res) + (in ? (mb + r) * a.e.ldr + n : 0), t);
+#pragma unroll
+          for (int j = 0; j < V; ++j) res[u * V + j] = t[j];
+        }
+      }
+      auto put = [&](auto* to, long long ld) __attribute__((always_inline)) {
+        using O = std::remove_pointer_t<decltype(to)>;
+#pragma unroll
+        for (int u = 0; u < kU; ++u) {
+          const int m = mb + first + u * kRows;
+          float t[V];
+#pragma unroll
+          for (int j = 0; j < V; ++j) t[j] = v[u * V + j];
+          if (on && m < a.M) store_pack<O, V>(to + m * ld + n, t);
+        }
+      };
+      if (slab) {
+        put(slab, a.N);
+        continue;
       }
 #pragma unroll
       for (int u = 0; u < kU; ++u) {
-        const int r = r0 + u * kRows, m = mb + r;
-        if (m >= a.M) continue;
-        float v[V];
-        load_pack<float, V>(turn + r * PITCH + c, v);
-        if (slab) store_pack<float, V>(slab + (long long)m * a.N + n, v);
-        else epilogue<S, V>(a.e, cols, m, n, v, res[u], ea[u]);
+        const int ea = sizeof(S) == 4 ? __shfl(ea32, first + u * kRows, 64) : 0;
+#pragma unroll
+        for (int j = 0; j < V; ++j) {
+          if constexpr (sizeof(S) == 4) v[u * V + j] = __builtin_ldexpf(v[u * V + j], ea + cols.eb[j]);
+          v[u * V + j] += cols.bias[j];
+        }
       }
+      if (a.e.z) put(static_cast<S*>(a.e.z), a.e.ldz);
+      act_of<sizeof(S) == 2, kU * V>(a.e.act, v);
+      if constexpr (RES)
+#pragma unroll
+        for (int j = 0; j < kU * V; ++j) v[j] += res[j];
+      put(static_cast<S*>(a.e.C), a.e.ldc);
     }
   }
 }
 
-// H: the products' type; S: the storage type of C, z, bias and residual (H, or float)
-template <typename H, typename S, bool AKC, bool BKC, int BM, int BN, int WM, int WN>
+// H: the products' type; S: the storage type of C, z, bias and residual (H, or float); RES: there is a residual
+template <typename H, typename S, bool AKC, bool BKC, bool RES, int BM, int BN, int WM, int WN>
 __global__ void __launch_bounds__(WM * WN * 64, BM == 256 && WM * WN == 4 ? 1 : 2) linear_gemm_kernel(const GemmArgs a) {
   constexpr int kTerms = __is_same(S, float) ? 3 : 1;
   constexpr int NW = WM * WN, TM = BM / WM, TN = BN / WN, FM = TM / 32, FN = TN / 32;
@@ -460,9 +494,11 @@ __global__ void __launch_bounds__(WM * WN * 64, BM == 256 && WM * WN == 4 ? 1 : 
     }
     __builtin_amdgcn_wave_barrier();   // a wave's LDS accesses are in order; the compiler's must be too
     const int mb = m0 + wm + 32 * j;
-    if (wide == 8) drain<S, 8, TN, kPitch>(a, slab, turn, lane, mb, n0 + wn);
-    else if (wide == 2) drain<S, 2, TN, kPitch>(a, slab, turn, lane, mb, n0 + wn);
-    else drain<S, 1, TN, kPitch>(a, slab, turn, lane, mb, n0 + wn);
+    // the powers of two of the slab's rows, one a lane
+    const int ea32 = sizeof(S) == 4 && a.e.ea && mb + (lane & 31) < a.M ? a.e.ea[mb + (lane & 31)] : 0;
+    if (wide == 8) drain<S, 8, RES, TN, kPitch>(a, slab, turn, lane, mb, n0 + wn, ea32);
+    else if (wide == 2) drain<S, 2, RES, TN, kPitch>(a, slab, turn, lane, mb, n0 + wn, ea32);
+    else drain<S, 1, RES, TN, kPitch>(a, slab, turn, lane, mb, n0 + wn, ea32);
     __builtin_amdgcn_wave_barrier();
   }
 }
@@ -492,7 +528,7 @@ __global__ void __launch_bounds__(256) linear_join_kernel(const GemmArgs a) {
 #pragma unroll
     for (int j = 0; j < V; ++j) res[j] = 0.f;
     if (a.e.res) load_pack<S, V>(static_cast<const S*>(a.e.res) + m * a.e.ldr + n, res);
-    epilogue<S, V>(a.e, cols, m, n, v, res, a.e.ea ? a.e.ea[m] : 0);
+    epilogue<S, V, true>(a.e, cols, m, n, v, res, a.e.ea ? a.e.ea[m] : 0);
   }
 }
 
@@ -573,7 +609,7 @@ __global__ void __launch_bounds__(1024) linear_few_kernel(const S* __restrict__ 
     Cols<S, 1> cols;
     cols.load(e, n);
     if (e.res) res[0] = (float)static_cast<const S*>(e.res)[m * e.ldr + n];
-    epilogue<S, 1>(e, cols, m, n, v, res, 0);
+    epilogue<S, 1, true>(e, cols, m, n, v, res, 0);
   }
 }
 
@@ -831,6 +867,14 @@ struct Pass {
     return m;
   }
 
+  template <typename H, typename S, bool AKC, bool BKC, bool RES>
+  void start(const GemmArgs& a, const Shape& c) {
+    const dim3 grid((unsigned)c.tiles, a.splits);
+    if (c.tile == 256)
+      hipLaunchKernelGGL((linear_gemm_kernel<H, S, AKC, BKC, RES, 256, 256, 2, 2>), grid, dim3(256), 0, st, a);
+    else
+      hipLaunchKernelGGL((linear_gemm_kernel<H, S, AKC, BKC, RES, 128, 128, 2, 2>), grid, dim3(256), 0, st, a);
+  }
   template <typename H, typename S, bool AKC, bool BKC>
   void product(const Mat& A, const Mat& B, int M, int N, int K, const Epi& e) {
     GemmArgs a{};
@@ -849,13 +893,13 @@ struct Pass {
     a.splits = (a.steps + a.per - 1) / a.per;
     if (a.splits > 1) a.slab = ws.take<float>((long long)a.splits * M * N);
     if (!run || rc != SE_OK) return;
-    const unsigned tiles = (unsigned)c.tiles;
-    if (c.tile == 256)
-      hipLaunchKernelGGL((linear_gemm_kernel<H, S, AKC, BKC, 256, 256, 2, 2>), dim3(tiles, a.splits), dim3(256), 0,
-                         st, a);
-    else
-      hipLaunchKernelGGL((linear_gemm_kernel<H, S, AKC, BKC, 128, 128, 2, 2>), dim3(tiles, a.splits), dim3(256), 0,
-                         st, a);
+    const bool res = e.res && a.splits == 1;
+    if constexpr (AKC && BKC) {   // the forward alone has one
+      if (res) start<H, S, AKC, BKC, true>(a, c);
+      else start<H, S, AKC, BKC, false>(a, c);
+    } else {
+      start<H, S, AKC, BKC, false>(a, c);
+    }
     launched();
     if (a.splits > 1) {
       // 8 columns a thread where the rows of everything are aligned for it
