@@ -273,25 +273,23 @@ __device__ __forceinline__ void tile_of(int id, int MT, int NT, int& mt, int& nt
 }
 
 // 32 rows of TN sums from `turn` through the epilogue (or into the slab), V columns a lane. Stores and loads complete in the
-// order they were asked for, so nothing in the loop may wait for a load behind a store: what the columns need is
-// there before it (`arrived`), a row's power of two comes from a register of another lane, and the residuals of eight
-// turns are asked for together.
-template <typename S, int V>
-__device__ __forceinline__ void arrived(const Cols<S, V>& c) {
-#pragma unroll
-  for (int j = 0; j < V; ++j) asm volatile("" ::"v"(c.bias[j]), "v"(c.eb[j]));
-}
+// order they were asked for, so the loop waits for no load behind a store but the residuals', eight turns' together.
 template <typename S, int V, bool RES, int TN, int PITCH>
-__device__ __forceinline__ void drain(const GemmArgs& a, float* slab, const float* turn, int lane, int mb, int nb, int ea32) {
+__device__ __forceinline__ void drain(const GemmArgs& a, float* slab, const float* turn, int lane, int mb, int nb,
+                                      const float* bias, const int* eb, const int* ea) {
   constexpr int kWide = TN < 64 * V ? TN : 64 * V, kLanes = kWide / V, kRows = 64 / kLanes;
   constexpr int kU = 32 / kRows < 8 ? 32 / kRows : 8;
 #pragma unroll 1
   for (int c0 = 0; c0 < TN; c0 += kWide) {
     const int c = c0 + (lane % kLanes) * V, n = nb + c;
     const bool on = n < a.N;   // V divides N
-    Cols<S, V> cols;
-    cols.load(a.e, on ? n : 0);
-    arrived(cols);
+    float cb[V];
+    int ce[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+      cb[j] = bias[c + j];
+      ce[j] = sizeof(S) == 4 ? eb[c + j] : 0;
+    }
 #pragma unroll 1
     for (int r0 = 0; r0 < 32; r0 += kU * kRows) {
       float v[kU * V], res[RES ? kU * V : 1];
@@ -326,14 +324,12 @@ __device__ __forceinline__ void drain(const GemmArgs& a, float* slab, const floa
         continue;
       }
 #pragma unroll
-      for (int u = 0; u < kU; ++u) {
-        const int ea = sizeof(S) == 4 ? __shfl(ea32, first + u * kRows, 64) : 0;
+      for (int u = 0; u < kU; ++u)
 #pragma unroll
         for (int j = 0; j < V; ++j) {
-          if constexpr (sizeof(S) == 4) v[u * V + j] = __builtin_ldexpf(v[u * V + j], ea + cols.eb[j]);
-          v[u * V + j] += cols.bias[j];
+          if constexpr (sizeof(S) == 4) v[u * V + j] = __builtin_ldexpf(v[u * V + j], ea[first + u * kRows] + ce[j]);
+          v[u * V + j] += cb[j];
         }
-      }
       if (a.e.z) put(static_cast<S*>(a.e.z), a.e.ldz);
       act_of<sizeof(S) == 2, kU * V>(a.e.act, v);
       if constexpr (RES)
@@ -352,6 +348,10 @@ __global__ void __launch_bounds__(WM * WN * 64, BM == 256 && WM * WN == 4 ? 1 : 
   using TA = Tile<AKC, BM, NW>;
   using TB = Tile<BKC, BN, NW>;
   __shared__ __attribute__((aligned(16))) u16 sA0[BM * kBK], sB0[BN * kBK], sA1[BM * kBK], sB1[BN * kBK];
+  // what the epilogue needs of its columns and rows: nothing may be waited for from memory behind the first store
+  constexpr bool f32 = sizeof(S) == 4;
+  __shared__ __attribute__((aligned(16))) float sBias[BN];
+  __shared__ __attribute__((aligned(16))) int sEb[f32 ? BN : 4], sEa[f32 ? BM : 4];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int MT = (a.M + BM - 1) / BM, NT = (a.N + BN - 1) / BN;
   int mt, nt;
@@ -359,6 +359,15 @@ __global__ void __launch_bounds__(WM * WN * 64, BM == 256 && WM * WN == 4 ? 1 : 
   const int m0 = mt * BM, n0 = nt * BN;
   const int wm = (wave % WM) * TM, wn = (wave / WM) * TN;
   const int s0 = blockIdx.y * a.per, s1 = min(a.steps, s0 + a.per);
+  if (!a.slab) {
+    for (int i = threadIdx.x; i < BN; i += NW * 64) {
+      const bool in = n0 + i < a.N;
+      sBias[i] = in && a.e.bias ? (float)static_cast<const S*>(a.e.bias)[n0 + i] : 0.f;
+      if constexpr (f32) sEb[i] = in && a.e.eb ? a.e.eb[n0 + i] - 2 * kTop : 0;
+    }
+    if constexpr (f32)
+      for (int i = threadIdx.x; i < BM; i += NW * 64) sEa[i] = m0 + i < a.M && a.e.ea ? a.e.ea[m0 + i] : 0;
+  }
   const unsigned offA = TA::lane_offset(lane, wave, a.lda), offB = TB::lane_offset(lane, wave, a.ldb);
 
   // where the tile after the one that is being loaded lies: its sources, and the lanes' offsets into them
@@ -494,11 +503,9 @@ __global__ void __launch_bounds__(WM * WN * 64, BM == 256 && WM * WN == 4 ? 1 : 
     }
     __builtin_amdgcn_wave_barrier();   // a wave's LDS accesses are in order; the compiler's must be too
     const int mb = m0 + wm + 32 * j;
-    // the powers of two of the slab's rows, one a lane
-    const int ea32 = sizeof(S) == 4 && a.e.ea && mb + (lane & 31) < a.M ? a.e.ea[mb + (lane & 31)] : 0;
-    if (wide == 8) drain<S, 8, RES, TN, kPitch>(a, slab, turn, lane, mb, n0 + wn, ea32);
-    else if (wide == 2) drain<S, 2, RES, TN, kPitch>(a, slab, turn, lane, mb, n0 + wn, ea32);
-    else drain<S, 1, RES, TN, kPitch>(a, slab, turn, lane, mb, n0 + wn, ea32);
+    if (wide == 8) drain<S, 8, RES, TN, kPitch>(a, slab, turn, lane, mb, n0 + wn, sBias + wn, sEb + wn, sEa + mb - m0);
+    else if (wide == 2) drain<S, 2, RES, TN, kPitch>(a, slab, turn, lane, mb, n0 + wn, sBias + wn, sEb + wn, sEa + mb - m0);
+    else drain<S, 1, RES, TN, kPitch>(a, slab, turn, lane, mb, n0 + wn, sBias + wn, sEb + wn, sEa + mb - m0);
     __builtin_amdgcn_wave_barrier();
   }
 }
@@ -779,9 +786,9 @@ inline int up8(int n) { return (n + 7) / 8 * 8; }
 inline unsigned blocks_for(long long n) { return (unsigned)std::min<long long>((n + 255) / 256, 8192); }
 
 // Tile and split of a product by what a round of workgroups costs, measured on 16384 x 8192 outputs over 2 to 128 steps of 64 k:
-// 256 x 256 tiles, one workgroup a CU, 20 us + 1.6 us a step; 128 x 128, two a CU, 6 us + 1.0 us a step. So large
-// tiles for long sums over many tiles (8192^3: 0.85 ms against 1.06), small ones for short sums and where their rounds fit
-// better (25792 x 2048 over 512: 88 us against 126). A split writes and reads its slabs at 4 bytes a sum.
+// 256 x 256 tiles, one workgroup a CU, 12 us + 1.52 us a step; 128 x 128, two a CU, 4.2 us + 0.97 us a step. So large
+// tiles for long sums over many tiles (8192^3: 0.83 ms against 1.02), small ones for short sums and where their rounds fit
+// better (25792 x 2048 over 512: 75 us against 94). A split's slabs are written and read at 4 bytes a sum.
 struct Shape {
   int tile, per;
   long long tiles;
@@ -791,14 +798,14 @@ inline Shape shape_of(int M, int N, int steps, int size) {
   double least = 1e300;
   for (int t : {128, 256}) {
     const long long tiles = (long long)((M + t - 1) / t) * ((N + t - 1) / t);
-    const double fixed = t == 256 ? 20 : 6, each = t == 256 ? 1.6 : 1.0, slots = t == 256 ? 256 : 512;
+    const double fixed = t == 256 ? 12 : 4.2, each = t == 256 ? 1.52 : 0.97, slots = t == 256 ? 256 : 512;
     for (int p = 1; p <= 64; p = p < 8 ? p + 1 : p + p / 4) {
       const int per = ((steps + p - 1) / p + 1) / 2 * 2;   // the kernel takes steps in pairs
       const int splits = (steps + per - 1) / per;
       if (p > 1 && (per < 4 || splits < 2)) break;
       const double rounds = std::ceil((double)tiles * splits / slots);
       double us = rounds * (fixed + each * per);
-      if (splits > 1) us += 4 + (double)M * N * (8.0 * splits + size) * 0.25e-6;
+      if (splits > 1) us += 3 + (double)M * N * (6.0 * splits + size) / 4.5e6;
       if (us < least) {
         least = us;
         best = Shape{t, per, tiles};
