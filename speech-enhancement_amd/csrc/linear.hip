@@ -786,7 +786,7 @@ inline int up8(int n) { return (n + 7) / 8 * 8; }
 inline unsigned blocks_for(long long n) { return (unsigned)std::min<long long>((n + 255) / 256, 8192); }
 
 // Tile and split of a product by what a round of workgroups costs, measured on 16384 x 8192 outputs over 2 to 128 steps of 64 k:
-// 256 x 256 tiles, one workgroup a CU, 12 us + 1.52 us a step; 128 x 128, two a CU, 4.2 us + 0.97 us a step. So large
+// 256 x 256 tiles, one workgroup a CU, 12 us + 1.52 us a step; 128 x 128, two a CU, 4.2 us + 0.97 us a step, alone on it 0.55 us. So large
 // tiles for long sums over many tiles (8192^3: 0.83 ms against 1.02), small ones for short sums and where their rounds fit
 // better (25792 x 2048 over 512: 75 us against 94). A split's slabs are written and read at 4 bytes a sum.
 struct Shape {
@@ -798,13 +798,16 @@ inline Shape shape_of(int M, int N, int steps, int size) {
   double least = 1e300;
   for (int t : {128, 256}) {
     const long long tiles = (long long)((M + t - 1) / t) * ((N + t - 1) / t);
-    const double fixed = t == 256 ? 12 : 4.2, each = t == 256 ? 1.52 : 0.97, slots = t == 256 ? 256 : 512;
+    const double fixed = t == 256 ? 12 : 4.2, each = t == 256 ? 1.52 : 0.97;
+    const long long slots = t == 256 ? 256 : 512;
     for (int p = 1; p <= 64; p = p < 8 ? p + 1 : p + p / 4) {
       const int per = ((steps + p - 1) / p + 1) / 2 * 2;   // the kernel takes steps in pairs
       const int splits = (steps + per - 1) / per;
       if (p > 1 && (per < 4 || splits < 2)) break;
-      const double rounds = std::ceil((double)tiles * splits / slots);
-      double us = rounds * (fixed + each * per);
+      const long long blocks = tiles * splits, rounds = blocks / slots, rest = blocks - rounds * slots;
+      // a last round that leaves every small tile a CU of its own steps faster
+      const double last = rest == 0 ? 0 : fixed + per * (t == 128 && rest <= 256 ? 0.55 : each);
+      double us = rounds * (fixed + each * per) + last;
       if (splits > 1) us += 3 + (double)M * N * (6.0 * splits + size) / 4.5e6;
       if (us < least) {
         least = us;
