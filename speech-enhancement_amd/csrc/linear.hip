@@ -12,10 +12,10 @@
 // ds_read_b64_tr_b16, which hands every lane four consecutive k of its own row. A direct load leaves lane l's
 // 16 bytes at l * 16, so the image is swizzled on the side of memory: which chunk of its row a lane fetches.
 //
-// fp32 storage: each operand is split beforehand into two fp16 planes x 2^(14 - e) = hi + lo (22 significant bits),
-// e from the largest magnitude of its own free index (a row of x has its own scale, so a loud frame costs a quiet one
-// no digits, and an infinity stays in its row), and the kernel walks k three times: hi hi, hi lo, lo hi; the
-// epilogue multiplies by 2^(ea + eb - 28).
+// fp32 storage: each operand is split beforehand into fp16 x 2^(14 - e) = hi + lo (22 significant bits), e from the
+// largest magnitude of its own free index (a row of x has its own scale, so a loud frame costs a quiet one no digits, and
+// an infinity stays in its row). 32 k of hi and the same 32 of lo lie side by side, 64 k of a tile, whose products are hi hi,
+// hi lo and lo hi; the epilogue multiplies by 2^(ea + eb - 28).
 #include "common.hpp"
 
 #include <algorithm>
@@ -47,14 +47,14 @@ struct Epi {
 };
 
 struct GemmArgs {
-  const u16* A[2];      // planes (one, or hi and lo)
-  const u16* B[2];
+  const u16* A;
+  const u16* B;
   long long lda, ldb;   // elements between the rows of the stored matrix
   long long a_bytes, b_bytes;
   float* slab;          // splits > 1: [splits][M][N]
   int M, N;             // rows of A and of B
-  int K, ksteps;        // reduced length, its tiles
-  int steps, per;       // terms * ksteps, and how many of them a split takes
+  int K;                // reduced length as it is stored (fp32: hi and lo)
+  int steps, per;       // its tiles, and how many of them a split takes
   int splits;
   Epi e;
 };
@@ -343,7 +343,6 @@ __device__ __forceinline__ void drain(const GemmArgs& a, float* slab, const floa
 // H: the products' type; S: the storage type of C, z, bias and residual (H, or float); RES: there is a residual
 template <typename H, typename S, bool AKC, bool BKC, bool RES, int BM, int BN, int WM, int WN>
 __global__ void __launch_bounds__(WM * WN * 64, BM == 256 && WM * WN == 4 ? 1 : 2) linear_gemm_kernel(const GemmArgs a) {
-  constexpr int kTerms = __is_same(S, float) ? 3 : 1;
   constexpr int NW = WM * WN, TM = BM / WM, TN = BN / WN, FM = TM / 32, FN = TN / 32;
   using TA = Tile<AKC, BM, NW>;
   using TB = Tile<BKC, BN, NW>;
@@ -376,10 +375,10 @@ __global__ void __launch_bounds__(WM * WN * 64, BM == 256 && WM * WN == 4 ? 1 : 
     unsigned oa, ob;
   } next;
   auto aim = [&](int s) __attribute__((always_inline)) {
-    const int term = kTerms == 1 ? 0 : s / a.ksteps, k0 = (s - term * a.ksteps) * kBK, kleft = a.K - k0;
+    const int k0 = s * kBK, kleft = a.K - k0;
     const bool on = s < s1;   // behind the last one: nothing is read
-    next.a = TA::source(a.A[term == 2], AKC ? m0 * a.lda + k0 : k0 * a.lda + m0, on ? a.a_bytes : 0);
-    next.b = TB::source(a.B[term == 1], BKC ? n0 * a.ldb + k0 : k0 * a.ldb + n0, on ? a.b_bytes : 0);
+    next.a = TA::source(a.A, AKC ? m0 * a.lda + k0 : k0 * a.lda + m0, on ? a.a_bytes : 0);
+    next.b = TB::source(a.B, BKC ? n0 * a.ldb + k0 : k0 * a.ldb + n0, on ? a.b_bytes : 0);
     // KC, behind the row's end: zeros
     next.oa = AKC && kleft < kBK && TA::lane_k(lane) >= kleft ? 0x80000000u : offA;
     next.ob = BKC && kleft < kBK && TB::lane_k(lane) >= kleft ? 0x80000000u : offB;
@@ -405,23 +404,26 @@ __global__ void __launch_bounds__(WM * WN * 64, BM == 256 && WM * WN == 4 ? 1 : 
   // The fragments of the next sixteen k are read while the matrix unit works on these; the last sixteen of a tile come
   // after the barrier that opens the next tile, so that its first fragments, and the loads into the tile just left,
   // are under way meanwhile.
-  s16x8 fa[2][FM], fb[2][FN];
-  auto read = [&](int set, const u16* la, const u16* lb, int kk) __attribute__((always_inline)) {
+  s16x8 fa[2][FM], fb[2][FN], fl[f32 ? FN : 1];
+  auto readA = [&](s16x8 (&f)[FM], const u16* la, int kk) __attribute__((always_inline)) {
 #pragma unroll
-    for (int i = 0; i < FN; ++i) fb[set][i] = TB::fragment(lb, wn + 32 * i, kk, lane);
-#pragma unroll
-    for (int j = 0; j < FM; ++j) fa[set][j] = TA::fragment(la, wm + 32 * j, kk, lane);
+    for (int j = 0; j < FM; ++j) f[j] = TA::fragment(la, wm + 32 * j, kk, lane);
   };
-  auto multiply = [&](int set) __attribute__((always_inline)) {
+  auto readB = [&](auto& f, const u16* lb, int kk) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < FN; ++i) f[i] = TB::fragment(lb, wn + 32 * i, kk, lane);
+  };
+  auto multiply = [&](const s16x8 (&f)[FM], const auto& g) __attribute__((always_inline)) {
 #pragma unroll
     for (int j = 0; j < FM; ++j)
 #pragma unroll
-      for (int i = 0; i < FN; ++i) acc[i][j] = mfma<H>(fb[set][i], fa[set][j], acc[i][j]);
+      for (int i = 0; i < FN; ++i) acc[i][j] = mfma<H>(g[i], f[j], acc[i][j]);
   };
   // LDS reads and loads between the products: all waves ask at the same time, and a wave whose requests wait their turn in
   // front of its products would start those late.
-  auto mixed = [&](auto loads) __attribute__((always_inline)) {
-    constexpr int kReads = FM * (AKC ? 1 : 2) + FN * (BKC ? 1 : 2), kProducts = FM * FN, kV = decltype(loads)::value;
+  constexpr int kReadA = FM * (AKC ? 1 : 2), kReadB = FN * (BKC ? 1 : 2);
+  auto mixed = [&](auto reads, auto loads) __attribute__((always_inline)) {
+    constexpr int kReads = decltype(reads)::value, kProducts = FM * FN, kV = decltype(loads)::value;
     constexpr int kEach = (kReads + kProducts - 1) / kProducts;
 #pragma unroll
     for (int i = 0; i < kProducts; ++i) {
@@ -434,31 +436,60 @@ __global__ void __launch_bounds__(WM * WN * 64, BM == 256 && WM * WN == 4 ? 1 : 
     __builtin_amdgcn_sched_barrier(0);
   };
   // The loads of a tile: the first part right after the barrier that frees its buffer, the rest over the next two steps, so
-  // that the last of them has a step's time until the barrier that waits for it.
+  // that the last of them has a step's time or more until the barrier that waits for it.
   constexpr int kL0 = (kLoads + 2) / 3, kL1 = kL0 + (kLoads - kL0 + 1) / 2;
   using N0 = std::integral_constant<int, kL0>;
   using N1 = std::integral_constant<int, kL1 - kL0>;
   using N2 = std::integral_constant<int, kLoads - kL1>;
+  using None = std::integral_constant<int, 0>;
+  using RA = std::integral_constant<int, kReadA>;
+  using RB = std::integral_constant<int, kReadB>;
+  using RAB = std::integral_constant<int, kReadA + kReadB>;
   // Tile s in (la, lb), its first fragments in set 0; tile s + 1 is on its way to (na, nb), whose first fragments are read at
-  // the end, when the loads of tile s + 2 into (la, lb) begin.
+  // the end (behind the last tile, for nothing), when the loads of tile s + 2 into (la, lb) begin.
   auto tile = [&](u16* la, u16* lb, u16* na, u16* nb, int s) __attribute__((always_inline)) {
-    load(kL0, kL1, na, nb);
-    read(1, la, lb, 16);
-    multiply(0);
-    mixed(N1{});
-    load(kL1, kLoads, na, nb);
-    read(0, la, lb, 32);
-    multiply(1);
-    mixed(N2{});
-    read(1, la, lb, 48);
-    multiply(0);
-    mixed(std::integral_constant<int, 0>{});
+    if constexpr (!f32) {
+      load(kL0, kL1, na, nb);
+      readA(fa[1], la, 16);
+      readB(fb[1], lb, 16);
+      multiply(fa[0], fb[0]);
+      mixed(RAB{}, N1{});
+      load(kL1, kLoads, na, nb);
+      readA(fa[0], la, 32);
+      readB(fb[0], lb, 32);
+      multiply(fa[1], fb[1]);
+      mixed(RAB{}, N2{});
+      readA(fa[1], la, 48);
+      readB(fb[1], lb, 48);
+      multiply(fa[0], fb[0]);
+      mixed(RAB{}, None{});
+    } else {   // hi of k 0 and 16 at 0 and 16, lo at 32 and 48; fa[0] and fb hold hi, fa[1] and fl lo
+      load(kL0, kL1, na, nb);
+      readB(fl, lb, 32);
+      multiply(fa[0], fb[0]);
+      mixed(RB{}, N1{});
+      load(kL1, kLoads, na, nb);
+      readA(fa[1], la, 32);
+      multiply(fa[0], fl);
+      mixed(RA{}, N2{});
+      readA(fa[0], la, 16);
+      readB(fb[1], lb, 16);
+      multiply(fa[1], fb[0]);
+      mixed(RAB{}, None{});
+      readB(fl, lb, 48);
+      multiply(fa[0], fb[1]);
+      mixed(RB{}, None{});
+      readA(fa[1], la, 48);
+      multiply(fa[0], fl);
+      mixed(RA{}, None{});
+    }
     aim(s + 2);
     __syncthreads();
     load(0, kL0, la, lb);
-    read(0, na, nb, 0);   // after the last tile nothing uses it
-    multiply(1);
-    mixed(N0{});
+    readA(fa[0], na, 0);
+    readB(fb[0], nb, 0);
+    multiply(fa[1], fb[1]);
+    mixed(RAB{}, N0{});
   };
 
   // two buffers of their own names, so that the compiler sees that a tile's loads do not touch the one being read
@@ -467,7 +498,8 @@ __global__ void __launch_bounds__(WM * WN * 64, BM == 256 && WM * WN == 4 ? 1 : 
   aim(s0 + 1);
   load(0, kL0, sA1, sB1);
   __syncthreads();
-  read(0, sA0, sB0, 0);
+  readA(fa[0], sA0, 0);
+  readB(fb[0], sB0, 0);
   for (int s = s0; s < s1; s += 2) {   // the tile behind an odd number of them is zeros
     tile(sA0, sB0, sA1, sB1, s);
     tile(sA1, sB1, sA0, sB0, s + 1);
@@ -647,26 +679,71 @@ __device__ __forceinline__ void split(float x, int e, _Float16& hi, _Float16& lo
   lo = fabsf(x) < INFINITY ? (_Float16)(s - (float)hi) : (_Float16)0.f;
 }
 
-// fp32 [R][C] at ld -> planes of rows Cp, one power of two a row (four rows a workgroup)
+// fp32 [R][C] at ld -> rows of 64 to each 32 columns (hi, then lo; zeros behind C), one power of two a row. A wave takes a row, a lane
+// pairs of columns; rows of up to 2048 stay in registers, longer ones are read again.
+constexpr int kSplitKeep = 16;
+template <bool TWO>
+__device__ __forceinline__ void load_two(const float* p, int c, int C, float& a, float& b) {
+  a = b = 0.f;
+  if (TWO && c + 1 < C) {
+    const float2 t = *reinterpret_cast<const float2*>(p + c);
+    a = t.x;
+    b = t.y;
+  } else {
+    if (c < C) a = p[c];
+    if (c + 1 < C) b = p[c + 1];
+  }
+}
+__device__ __forceinline__ void split_two(float a, float b, int ea, int eb, unsigned& hi, unsigned& lo) {
+  typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+  _Float16 h0, l0, h1, l1;
+  split(a, ea, h0, l0);
+  split(b, eb, h1, l1);
+  hi = __builtin_bit_cast(unsigned, (f16x2){h0, h1});
+  lo = __builtin_bit_cast(unsigned, (f16x2){l0, l1});
+}
+template <bool TWO>
 __global__ void __launch_bounds__(256) linear_split_rows_kernel(const float* __restrict__ x, long long ld, int R, int C,
-                                                                int Cp, _Float16* __restrict__ hi,
-                                                                _Float16* __restrict__ lo, short* __restrict__ ex) {
-  const int r = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
+                                                                int C32, unsigned* __restrict__ out,
+                                                                short* __restrict__ ex) {
+  const long long r = blockIdx.x * 4LL + (threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63;
   if (r >= R) return;
   const float* p = x + r * ld;
-  float m = 0.f;
-  for (int c = lane; c < C; c += 64) m = fmaxf(m, finite_abs(p[c]));
+  unsigned* o = out + r * C32;   // C32 pairs of words: 2 C32 halves
+  float v[kSplitKeep][2], m = 0.f;
+#pragma unroll
+  for (int i = 0; i < kSplitKeep; ++i) {
+    v[i][0] = v[i][1] = 0.f;
+    if (i * 128 < C) load_two<TWO>(p, i * 128 + 2 * lane, C, v[i][0], v[i][1]);
+    m = fmaxf(m, fmaxf(finite_abs(v[i][0]), finite_abs(v[i][1])));
+  }
+  for (int c = kSplitKeep * 128 + 2 * lane; c < C; c += 128) {
+    float a, b;
+    load_two<TWO>(p, c, C, a, b);
+    m = fmaxf(m, fmaxf(finite_abs(a), finite_abs(b)));
+  }
   const int e = exp_of(se::wave_max(m));
   if (lane == 0) ex[r] = (short)e;
-  for (int c = lane; c < Cp; c += 64) {
-    _Float16 h, l;
-    split(c < C ? p[c] : 0.f, e, h, l);
-    hi[(long long)r * Cp + c] = h;
-    lo[(long long)r * Cp + c] = l;
+  auto put = [&](int c, float a, float b) __attribute__((always_inline)) {
+    unsigned hi, lo;
+    split_two(a, b, e, e, hi, lo);
+    const int at = (c >> 5) * 32 + (c & 31) / 2;
+    o[at] = hi;
+    o[at + 16] = lo;
+  };
+#pragma unroll
+  for (int i = 0; i < kSplitKeep; ++i)
+    if (i * 128 + 2 * lane < C32) put(i * 128 + 2 * lane, v[i][0], v[i][1]);
+  for (int c = kSplitKeep * 128 + 2 * lane; c < C32; c += 128) {
+    float a, b;
+    load_two<TWO>(p, c, C, a, b);
+    put(c, a, b);
   }
 }
 
-// the same with one power of two a column: the columns' largest magnitudes over chunks of rows, then the planes
+// the same with one power of two a column, 32 rows of hi, then the 32 of lo: the columns' largest magnitudes over chunks
+// of rows, their powers, then the halves in rows of Cp
 __global__ void __launch_bounds__(256) linear_col_max_kernel(const float* __restrict__ x, long long ld, int R, int C,
                                                              int rows, float* __restrict__ part) {
   const int c = blockIdx.x * 256 + threadIdx.x;
@@ -677,25 +754,35 @@ __global__ void __launch_bounds__(256) linear_col_max_kernel(const float* __rest
   for (int r = r0; r < r1; ++r) m = fmaxf(m, finite_abs(x[r * ld + c]));
   part[(long long)blockIdx.y * C + c] = m;
 }
-__global__ void __launch_bounds__(256) linear_col_exp_kernel(const float* __restrict__ part, int parts, int C,
-                                                             short* __restrict__ ex) {
-  const int c = blockIdx.x * 256 + threadIdx.x;
-  if (c >= C) return;
+__global__ void __launch_bounds__(1024) linear_col_exp_kernel(const float* __restrict__ part, int parts, int C,
+                                                              short* __restrict__ ex) {
+  __shared__ float s[16][64];
+  const int l = threadIdx.x & 63, k = threadIdx.x >> 6, c = blockIdx.x * 64 + l;
   float m = 0.f;
+  if (c < C)
 #pragma unroll 8
-  for (int i = 0; i < parts; ++i) m = fmaxf(m, part[(long long)i * C + c]);
+    for (int i = k; i < parts; i += 16) m = fmaxf(m, part[(long long)i * C + c]);
+  s[k][l] = m;
+  __syncthreads();
+  if (k || c >= C) return;
+  for (int i = 1; i < 16; ++i) m = fmaxf(m, s[i][l]);
   ex[c] = (short)exp_of(m);
 }
-__global__ void __launch_bounds__(256) linear_split_cols_kernel(const float* __restrict__ x, long long ld, int R, int C,
+template <bool TWO>
+__global__ void __launch_bounds__(256) linear_split_cols_kernel(const float* __restrict__ x, long long ld, int R, int R32, int C,
                                                                 int Cp, const short* __restrict__ ex,
-                                                                _Float16* __restrict__ hi, _Float16* __restrict__ lo) {
-  const long long total = (long long)R * Cp;
+                                                                unsigned* __restrict__ out) {
+  const int per = Cp / 2;
+  const long long total = (long long)R32 * per;
   for (long long i = blockIdx.x * 256LL + threadIdx.x; i < total; i += gridDim.x * 256LL) {
-    const int r = (int)(i / Cp), c = (int)(i - (long long)r * Cp);
-    _Float16 h, l;
-    split(c < C ? x[r * ld + c] : 0.f, c < C ? ex[c] : 0, h, l);
-    hi[i] = h;
-    lo[i] = l;
+    const int r = (int)(i / per), c = (int)(i - (long long)r * per) * 2;
+    float a = 0.f, b = 0.f;
+    if (r < R) load_two<TWO>(x + r * ld, c, C, a, b);
+    unsigned hi, lo;
+    split_two(a, b, c < C ? ex[c] : 0, c + 1 < C ? ex[c + 1] : 0, hi, lo);
+    const long long at = ((long long)(r >> 5) * 64 + (r & 31)) * per + c / 2;
+    out[at] = hi;
+    out[at + 32LL * per] = lo;
   }
 }
 
@@ -777,7 +864,7 @@ struct Carve {   // a workspace, or (base NULL) its size
 };
 
 struct Mat {            // an operand as the kernel reads it
-  const u16* p[2];
+  const u16* p;
   const short* ex;
   long long ld, bytes;
 };
@@ -793,12 +880,12 @@ struct Shape {
   int tile, per;
   long long tiles;
 };
-inline Shape shape_of(int M, int N, int steps, int size) {
+inline Shape shape_of(int M, int N, int steps, double products) {   // products: of a step, against 16 bits
   Shape best{};
   double least = 1e300;
   for (int t : {128, 256}) {
     const long long tiles = (long long)((M + t - 1) / t) * ((N + t - 1) / t);
-    const double fixed = t == 256 ? 12 : 4.2, each = t == 256 ? 1.52 : 0.97;
+    const double fixed = (t == 256 ? 12 : 4.2) * products, each = (t == 256 ? 1.52 : 0.97) * products;
     const long long slots = t == 256 ? 256 : 512;
     for (int p = 1; p <= 64; p = p < 8 ? p + 1 : p + p / 4) {
       const int per = ((steps + p - 1) / p + 1) / 2 * 2;   // the kernel takes steps in pairs
@@ -806,9 +893,9 @@ inline Shape shape_of(int M, int N, int steps, int size) {
       if (p > 1 && (per < 4 || splits < 2)) break;
       const long long blocks = tiles * splits, rounds = blocks / slots, rest = blocks - rounds * slots;
       // a last round that leaves every small tile a CU of its own steps faster
-      const double last = rest == 0 ? 0 : fixed + per * (t == 128 && rest <= 256 ? 0.55 : each);
+      const double last = rest == 0 ? 0 : fixed + per * (t == 128 && rest <= 256 ? 0.55 * products : each);
       double us = rounds * (fixed + each * per) + last;
-      if (splits > 1) us += 3 + (double)M * N * (6.0 * splits + size) / 4.5e6;
+      if (splits > 1) us += 3 + (double)M * N * (6.0 * splits + 2) / 4.5e6;
       if (us < least) {
         least = us;
         best = Shape{t, per, tiles};
@@ -832,7 +919,7 @@ struct Pass {
   Mat half(const void* x, long long ld, int R, int C) {
     Mat m{};
     if (ld % 8 == 0 && C % 8 == 0 && ((uintptr_t)x & 15) == 0) {
-      m.p[0] = static_cast<const u16*>(x);
+      m.p = static_cast<const u16*>(x);
       m.ld = ld;
       m.bytes = ((long long)(R - 1) * ld + C) * 2;
       return m;
@@ -844,36 +931,39 @@ struct Pass {
                          static_cast<const u16*>(x), ld, R, C, Cp, out);
       launched();
     }
-    m.p[0] = out;
+    m.p = out;
     m.ld = Cp;
     m.bytes = (long long)R * Cp * 2;
     return m;
   }
-  // fp32 [R][C] at ld as two planes, powers of two by row or by column
+  // fp32 [R][C] at ld as hi and lo, powers of two by row (reduced along the row) or by column (along the column)
   Mat planes(const void* xv, long long ld, int R, int C, bool by_row) {
     const float* x = static_cast<const float*>(xv);
+    const bool two = ld % 2 == 0 && ((uintptr_t)x & 7) == 0;
+    const int C32 = (C + 31) / 32 * 32, R32 = (R + 31) / 32 * 32, Cp = up8(C);
     Mat m{};
-    const int Cp = up8(C);
-    _Float16* hi = ws.take<_Float16>((long long)R * Cp);
-    _Float16* lo = ws.take<_Float16>((long long)R * Cp);
+    m.ld = by_row ? 2LL * C32 : Cp;
+    m.bytes = (by_row ? (long long)R : 2LL * R32) * m.ld * 2;
+    u16* out = ws.take<u16>(m.bytes / 2);
     short* ex = ws.take<short>(by_row ? R : C);
+    m.p = out;
+    m.ex = ex;
     const int rows = std::max(64, (R + 255) / 256), parts = (R + rows - 1) / rows;
     float* part = by_row ? nullptr : ws.take<float>((long long)parts * C);
-    if (run && by_row) {
-      hipLaunchKernelGGL(linear_split_rows_kernel, dim3((R + 3) / 4), dim3(256), 0, st, x, ld, R, C, Cp, hi, lo, ex);
-      launched();
-    } else if (run) {
+    if (!run) return m;
+    unsigned* to = reinterpret_cast<unsigned*>(out);
+    if (by_row) {
+      const dim3 grid((R + 3LL) / 4);
+      if (two) hipLaunchKernelGGL(linear_split_rows_kernel<true>, grid, dim3(256), 0, st, x, ld, R, C, C32, to, ex);
+      else hipLaunchKernelGGL(linear_split_rows_kernel<false>, grid, dim3(256), 0, st, x, ld, R, C, C32, to, ex);
+    } else {
       hipLaunchKernelGGL(linear_col_max_kernel, dim3((C + 255) / 256, parts), dim3(256), 0, st, x, ld, R, C, rows, part);
-      hipLaunchKernelGGL(linear_col_exp_kernel, dim3((C + 255) / 256), dim3(256), 0, st, part, parts, C, ex);
-      hipLaunchKernelGGL(linear_split_cols_kernel, dim3(blocks_for((long long)R * Cp)), dim3(256), 0, st, x, ld, R, C,
-                         Cp, ex, hi, lo);
-      launched();
+      hipLaunchKernelGGL(linear_col_exp_kernel, dim3((C + 63) / 64), dim3(1024), 0, st, part, parts, C, ex);
+      const dim3 grid(blocks_for((long long)R32 * Cp / 2));
+      if (two) hipLaunchKernelGGL(linear_split_cols_kernel<true>, grid, dim3(256), 0, st, x, ld, R, R32, C, Cp, ex, to);
+      else hipLaunchKernelGGL(linear_split_cols_kernel<false>, grid, dim3(256), 0, st, x, ld, R, R32, C, Cp, ex, to);
     }
-    m.p[0] = reinterpret_cast<const u16*>(hi);
-    m.p[1] = reinterpret_cast<const u16*>(lo);
-    m.ex = ex;
-    m.ld = Cp;
-    m.bytes = (long long)R * Cp * 2;
+    launched();
     return m;
   }
 
@@ -890,14 +980,16 @@ struct Pass {
     GemmArgs a{};
     a.M = M; a.N = N; a.K = K;
     a.lda = A.ld; a.ldb = B.ld; a.a_bytes = A.bytes; a.b_bytes = B.bytes;
-    for (int i = 0; i < 2; ++i) { a.A[i] = A.p[i]; a.B[i] = B.p[i]; }
+    a.A = A.p; a.B = B.p;
     a.e = e;
     a.e.ea = A.ex; a.e.eb = B.ex;
-    a.ksteps = (K + kBK - 1) / kBK;
-    const long long steps = (long long)(__is_same(S, float) ? 3 : 1) * a.ksteps;
-    if (steps > 0x3fffffffLL || A.ld > (1 << 21) || B.ld > (1 << 21)) { rc = SE_E_UNSUPPORTED; return; }
-    a.steps = (int)steps;
-    const Shape c = shape_of(M, N, a.steps, sizeof(S));
+    if (__is_same(S, float)) {   // 32 k of hi and of lo to a tile
+      if (K > (1 << 29)) { rc = SE_E_UNSUPPORTED; return; }
+      a.K = 2 * ((K + 31) / 32 * 32);
+    }
+    if (A.ld > (1 << 22) || B.ld > (1 << 22)) { rc = SE_E_UNSUPPORTED; return; }
+    a.steps = (a.K + kBK - 1) / kBK;
+    const Shape c = shape_of(M, N, a.steps, sizeof(S) == 4 ? 1.5 : 1);
     if (c.tiles > 0x7fffffffLL) { rc = SE_E_UNSUPPORTED; return; }
     a.per = c.per;
     a.splits = (a.steps + a.per - 1) / a.per;
