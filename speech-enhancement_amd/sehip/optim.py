@@ -247,7 +247,9 @@ def _multi(params, columns, types, bits, step, lr, betas, eps, weight_decay, see
         if (list(map(T.numel, ts)) != want or set(map(_dtype_of, ts)) != {ty} or set(map(T.get_device, ts)) != {index}
                 or not all(map(T.is_contiguous, ts))):
             raise RuntimeError(f"sehip adamw: {name}: not all contiguous {ty} tensors of the parameters' sizes on {dev}")
-        arr[name] = list(map(T.data_ptr, ts))
+        arr[name] = at = list(map(T.data_ptr, ts))
+        if name != "grad" and len(set(at)) < n and len({a for a, k in zip(at, sizes) if k}) < sum(map(bool, sizes)):
+            raise RuntimeError(f"sehip adamw: the same {name} twice in the list")
     arr["numel"] = sizes
     if torch.cuda.is_current_stream_capturing():
         raise RuntimeError("sehip adamw: a captured graph would repeat this step's count and bias corrections")

@@ -333,6 +333,12 @@ def test_refusals_on_the_gpu(gpu_device):
                 optim.adamw32_(*args, **kw)
     with pytest.raises(RuntimeError, match="sehip adamw"):
         optim.adamw8_([f()], [f()], [f()], [f(1)], [f()], [f(1)], **kw)
+    p, m = f(), f()
+    with pytest.raises(RuntimeError, match="twice"):   # two chunks of one launch would update the same memory
+        optim.adamw32_([p, p], [f(), f()], [f(), f()], [f(), f()], **kw)
+    with pytest.raises(RuntimeError, match="twice"):
+        optim.adamw32_([f(), f()], [f(), f()], [m, m], [f(), f()], **kw)
+    optim.adamw32_([f(0), f(0), f()], [f(0), f(0), p], [f(0), f(0), f()], [f(0), f(0), f()], **kw)
     torch.cuda.synchronize()
     g = torch.cuda.CUDAGraph()
     t = [[f()], [f()], [f()], [f()]]
@@ -340,6 +346,28 @@ def test_refusals_on_the_gpu(gpu_device):
         with torch.cuda.graph(g):
             t[0][0].add_(1)
             optim.adamw32_(*t, **kw)
+
+
+@pytest.mark.parametrize("bits", (8, 32))
+def test_train_step_of_a_model(gpu_device, bits):
+    """FRCRN's own training step (sehip.train.train_step) on the 8- and 32-bit states, over its 279 parameter tensors: 32 bits
+    gives the default optimizer's parameters (the same fp32 formula: 1e-6 of the largest, as elsewhere in this suite), 8 bits
+    the same first step to that bar (its moments start at zero, and the step is taken before they are rounded)."""
+    import paramfill
+    from sehip import models as M
+    from sehip.train import make_optimizer, train_step
+    noisy, clean = paramfill.structured_pair(2, 16000, seed=11)
+    x, c = torch.from_numpy(noisy).to(gpu_device), torch.from_numpy(clean).to(gpu_device)
+    ms = [paramfill.fill_(M.FRCRN(), seed=12).to(gpu_device).train() for _ in range(2)]
+    opts = [make_optimizer(ms[0]), make_optimizer(ms[1], state_bits=bits)]
+    for m, o in zip(ms, opts):
+        assert torch.isfinite(train_step(m, o, x, c))
+    for p, q in zip(ms[0].parameters(), ms[1].parameters()):
+        assert (p - q).abs().max().item() <= 1e-6 * max(p.abs().max().item(), 1e-2)
+    assert torch.isfinite(train_step(ms[1], opts[1], x, c))
+    held = sum(t.numel() * t.element_size() for st in opts[1].state.values() for t in st.values() if t.is_cuda)
+    total = sum(p.numel() for p in ms[1].parameters())
+    assert held == 8 * total if bits == 32 else held < 2.1 * total
 
 
 @pytest.mark.parametrize("dt,bits", [(torch.float32, 8), (torch.bfloat16, 32), (torch.bfloat16, 8)])
