@@ -801,11 +801,13 @@ int se_layer_norm_bwd(const void* dy, long long dy_stride, const void* x, long l
  * residual add): z = x W^T + bias, y = act(z) + residual.
  * x [M, K] rows ldx apart, w [N, K] rows ldw apart, residual [M, N] rows ldr
  * apart (or NULL), y dense [M, N]; z (or NULL) receives the pre-activation for the
- * backward, rows ceil(N / 8) * 8 apart, on 16 bytes. All of one storage type; fp32 accumulation, y rounded once.
+ * backward, rows ceil(N / 8) * 8 apart, on 16 bytes. All of one storage type;
+ * fp32 accumulation, y rounded once.
  * Backward: g = dy act'(z) (dy's rows ldr apart), dx = g W, dw = g^T x,
  * db = sum_m g; what is not NULL is written, z is needed where act is not
- * SE_LINACT_NONE. The workspace sizes depend on the pointers' alignment; the
- * forward of up to SE_LINEAR_FEW_ROWS rows takes none.
+ * SE_LINACT_NONE. N, K and the strides up to 2^21, M up to 2^28, each matrix up
+ * to 2^37 elements; more is SE_E_UNSUPPORTED. The workspace sizes depend on the
+ * pointers' alignment; the forward of up to SE_LINEAR_FEW_ROWS rows takes none.
  * ------------------------------------------------------------------------ */
 enum {
   SE_LINACT_NONE = 0,

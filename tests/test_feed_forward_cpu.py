@@ -80,6 +80,20 @@ def test_linear_c_arguments():
     assert bwd(ctypes.byref(d), p, p, p, p, p, p, p, None, 0, None) == -5
 
 
+@pytest.mark.parametrize("m,n,k", [((1 << 28) + 1, 4, 8), ((1 << 31) - 1, 1, 1), (1 << 28, 1 << 10, 8),
+                                   (1 << 28, 8, 1 << 10), (70, 1 << 21, 1 << 17)])
+def test_linear_sizes_behind_32_bits(m, n, k):
+    """Refused before anything is launched: row indexes are 32-bit and a launch has less than 2^32 threads."""
+    lib = N.lib()
+    p = ctypes.c_void_p(256)
+    for dt in range(3):
+        d = N.LinearDesc(m, n, k, 0, dt, k, k, n)
+        assert lib.se_linear_fwd(ctypes.byref(d), p, p, None, None, p, None, None, 0, None) == -3
+        assert lib.se_linear_bwd(ctypes.byref(d), p, p, p, None, p, p, p, None, 0, None) == -3
+        assert lib.se_linear_fwd_workspace_size(ctypes.byref(d), p, p) == 0
+        assert lib.se_linear_bwd_workspace_size(ctypes.byref(d), p, p, p, 1, 1, 1) == 0
+
+
 def _lists(n=(5,), **over):
     def codes(k, t):
         return torch.zeros(k, dtype=torch.uint8).view(t)
