@@ -14,8 +14,8 @@
 //
 // Bound by memory: at 8 bits an element of an fp32 parameter reads and writes 16.06 bytes. The table of tensors goes in
 // the kernel's arguments (no copy, no device table to keep alive, 48 tensors a launch); a workgroup takes one
-// chunk of 2048 consecutive elements of one tensor, eight a thread, so 16 lanes share a block's exponent. The large
-// 8-bit case of fp32 parameters: 1.0 ms, 5.4 TB/s (a large copy: 5.0); bf16 parameters with 32-bit states: 297 us, 5.0.
+// chunk of 2048 consecutive elements of one tensor, eight a thread, so 16 lanes share a block's exponent. 336 M fp32
+// parameters with 8-bit states: 1.05 ms, 5.1 TB/s (a large copy: 5.0); 67 M bf16 ones with 32-bit states: 297 us, 5.0.
 #include "common.hpp"
 
 #include <cmath>
@@ -44,6 +44,7 @@ struct Table {
 };
 struct Hyper {
   float decay, w1, b2, omb2, inv_bc2_sqrt, eps, neg_step;
+  float w1_lo, b2_lo, omb2_lo;   // what the 32 bits of each leave over
 };
 static_assert(sizeof(Table) + sizeof(Hyper) <= 4096, "kernel arguments");
 
@@ -108,6 +109,41 @@ __device__ __forceinline__ void load_codes(const unsigned char* p, bool vec, int
   }
 }
 
+// A code is a step function of the state and of h, and the errors of 32-bit arithmetic turn about one in a million, that lies
+// next to its border. A code within kNear of one is taken again from the state as hi + lo, lo what hi's rounding
+// left over: the products' and sums' errors by fma and by the two-sum of Knuth, q's from s - q^2 = 2 q lo.
+// 336 M parameters in 1.05 ms against 1.02 without; every state in twice the bits took 1.26, the flagged waves'
+// states all eight again 1.15 (95 registers, five waves a SIMD).
+constexpr float kNear = 0x1p-17f;   // the errors: a few 2^-24 of a value of up to 16
+__device__ __forceinline__ void two_sum(float a, float b, float& s, float& e) {
+#pragma clang fp contract(off)
+  s = a + b;
+  const float t = s - a;
+  e = (a - (s - t)) + (b - t);
+}
+__device__ __forceinline__ void step_m(const Hyper& h, float g, float& m, float& lo) {
+#pragma clang fp contract(off)
+  float d, ed, s, es;
+  two_sum(g, -m, d, ed);
+  const float p = h.w1 * d;
+  two_sum(m, p, s, es);
+  lo = es + (__builtin_fmaf(h.w1, d, -p) + __builtin_fmaf(h.w1, ed, h.w1_lo * d));
+  m = s;
+}
+// v: q^2 on entry (q of 4 bits: exact), q on return
+__device__ __forceinline__ void step_q(const Hyper& h, float g, float& v, float& lo) {
+#pragma clang fp contract(off)
+  const float a = h.b2 * v, gg = g * g, c = h.omb2 * gg;
+  float s, es;
+  two_sum(a, c, s, es);
+  const float ea = __builtin_fmaf(h.b2, v, -a) + h.b2_lo * v;
+  const float ec = __builtin_fmaf(h.omb2, gg, -c);
+  const float eg = __builtin_fmaf(h.omb2, __builtin_fmaf(g, g, -gg), h.omb2_lo * gg);
+  const float q = sqrtf(s);
+  lo = q > 0.f ? (__builtin_fmaf(-q, q, s) + (es + (ea + (ec + eg)))) * 0.5f * __builtin_amdgcn_rcpf(q) : 0.f;
+  v = q;
+}
+
 // k + 127 of the block that this thread's sixteen lanes hold: amax over their finite values
 __device__ __forceinline__ unsigned block_exp(const float (&v)[8]) {
   float m = 0.f;
@@ -123,28 +159,39 @@ __device__ __forceinline__ unsigned block_exp(const float (&v)[8]) {
   return (unsigned)max(k, 1);
 }
 
-// e4m3 code of x 2^-k, rounded stochastically by the 16 bits h; NaN for what is not finite
-__device__ __forceinline__ unsigned code_of(float x, float inv, unsigned h, bool floor1) {
+// e4m3 code of x 2^-k, rounded stochastically by the 16 bits h; NaN for what is not finite. EXACT: of x + lo
+template <bool EXACT>
+__device__ __forceinline__ unsigned code_of(float x, float lo, float inv, unsigned h, bool floor1, bool& near) {
+#pragma clang fp contract(off)
   const float a = fabsf(x);
   const float y = a * inv;
   const int e = max((int)(__builtin_bit_cast(unsigned, y) >> 23) - 127, -6);
-  const float f = floorf(__builtin_ldexpf(y, 3 - e) + ((float)h + 0.5f) * 0x1p-16f);   // 8 .. 16, or less below 2^-6
+  const float z = __builtin_ldexpf(y, 3 - e), u = ((float)h + 0.5f) * 0x1p-16f;   // z: 8 .. 16, or less below 2^-6
+  float f;
+  if constexpr (EXACT) {
+    float t, et;
+    two_sum(z, u, t, et);
+    f = floorf(t);
+    if (f == t && et + __builtin_ldexpf((x < 0.f ? -lo : lo) * inv, 3 - e) < 0.f) f -= 1.f;   // a little below f
+  } else {
+    const float t = z + u;
+    f = floorf(t);
+    near = fabsf(t - rintf(t)) < kNear;
+  }
   unsigned c = (unsigned)(((e + 7) << 3) + (int)f - 8);
   if (floor1 && a > 0.f) c = max(c, 1u);
   if (!(a < INFINITY)) c = 0x7fu;
   return c | ((__builtin_bit_cast(unsigned, x) >> 24) & 0x80u);
 }
 
-__device__ __forceinline__ void store_codes(unsigned char* p, bool vec, int left, const unsigned (&c)[8]) {
+// eight codes in two words
+__device__ __forceinline__ void store_codes(unsigned char* p, bool vec, int left, unsigned w0, unsigned w1) {
   if (vec && left >= 8) {
-    uint2 t;
-    t.x = c[0] | c[1] << 8 | c[2] << 16 | c[3] << 24;
-    t.y = c[4] | c[5] << 8 | c[6] << 16 | c[7] << 24;
-    *reinterpret_cast<uint2*>(p) = t;
+    *reinterpret_cast<uint2*>(p) = uint2{w0, w1};
   } else {
 #pragma unroll
     for (int j = 0; j < 8; ++j)
-      if (j < left) p[j] = (unsigned char)c[j];
+      if (j < left) p[j] = (unsigned char)((j < 4 ? w0 : w1) >> (8 * (j & 3)));
   }
 }
 
@@ -164,8 +211,8 @@ __global__ void __launch_bounds__(kThr) adamw_multi_kernel(const Table tab, cons
   float p[8], g[8], m[8], v[8];
   load8(P, vec, left, p);
   load8(static_cast<const T*>(t.g) + i, vec, left, g);
+  unsigned mk = 1u, vk = 1u;
   if constexpr (Q8) {
-    unsigned mk = 1u, vk = 1u;
     if (left > 0) {
       mk = max((unsigned)t.mk[i / kBlock], 1u);
       vk = max((unsigned)t.vk[i / kBlock], 1u);
@@ -188,21 +235,49 @@ __global__ void __launch_bounds__(kThr) adamw_multi_kernel(const Table tab, cons
   }
   store8(P, vec, left, p);
   if constexpr (Q8) {
-    const unsigned mk = block_exp(m), vk = block_exp(v);
-    const float mi = __builtin_bit_cast(float, (254u - mk) << 23), vi = __builtin_bit_cast(float, (254u - vk) << 23);
     const unsigned base = (unsigned)i * 0x9E3779B1u + (unsigned)(i >> 32) * 0x243F6A89u + t.key;
-    unsigned cm[8], cv[8];
+    const unsigned nmk = block_exp(m), nvk = block_exp(v);
+    const float mi = __builtin_bit_cast(float, (254u - nmk) << 23), vi = __builtin_bit_cast(float, (254u - nvk) << 23);
+    unsigned char* cm = static_cast<unsigned char*>(t.m) + i;
+    unsigned char* cv = static_cast<unsigned char*>(t.v) + i;
+    unsigned wm[2] = {0u, 0u}, wv[2] = {0u, 0u}, again = 0;
 #pragma unroll
     for (int j = 0; j < 8; ++j) {   // i is a multiple of 8: the upper half is the same for all eight
       const unsigned r = mix(base + j * 0x9E3779B1u);
-      cm[j] = code_of(m[j], mi, r & 0xffffu, false);
-      cv[j] = code_of(v[j], vi, r >> 16, true);
+      bool nm, nv;
+      wm[j >> 2] |= code_of<false>(m[j], 0.f, mi, r & 0xffffu, false, nm) << (8 * (j & 3));
+      wv[j >> 2] |= code_of<false>(v[j], 0.f, vi, r >> 16, true, nv) << (8 * (j & 3));
+      again |= (j < left && (nm || nv)) ? 1u << j : 0u;
     }
-    store_codes(static_cast<unsigned char*>(t.m) + i, vec, left, cm);
-    store_codes(static_cast<unsigned char*>(t.v) + i, vec, left, cv);
+    while (again) {   // one element in thirty thousand: its codes are still in memory
+      const int j = __builtin_ctz(again);
+      again &= again - 1;
+      const unsigned r = mix(base + j * 0x9E3779B1u);
+      const float gj = (float)static_cast<const T*>(t.g)[i + j];
+      float mj = __builtin_amdgcn_cvt_f32_fp8((int)cm[j], 0) * __builtin_bit_cast(float, mk << 23);
+      float vj = __builtin_amdgcn_cvt_f32_fp8((int)cv[j], 0) * __builtin_bit_cast(float, vk << 23);
+      float ml, vl;
+      bool n;
+      vj *= vj;
+      step_m(h, gj, mj, ml);
+      step_q(h, gj, vj, vl);
+      const int at = 8 * (j & 3);
+      const unsigned keep = ~(0xffu << at);
+      const unsigned a = code_of<true>(mj, ml, mi, r & 0xffffu, false, n) << at;
+      const unsigned b = code_of<true>(vj, vl, vi, r >> 16, true, n) << at;
+      if (j < 4) {
+        wm[0] = (wm[0] & keep) | a;
+        wv[0] = (wv[0] & keep) | b;
+      } else {
+        wm[1] = (wm[1] & keep) | a;
+        wv[1] = (wv[1] & keep) | b;
+      }
+    }
+    store_codes(cm, vec, left, wm[0], wm[1]);
+    store_codes(cv, vec, left, wv[0], wv[1]);
     if (left > 0 && (threadIdx.x & 15) == 0) {
-      t.mk[i / kBlock] = (unsigned char)mk;
-      t.vk[i / kBlock] = (unsigned char)vk;
+      t.mk[i / kBlock] = (unsigned char)nmk;
+      t.vk[i / kBlock] = (unsigned char)nvk;
     }
   } else {
     store8(static_cast<float*>(t.m) + i, vec, left, m);
@@ -238,6 +313,9 @@ extern "C" int se_adamw_multi(const se_adamw_tensor* tensors, int n, int dtype, 
   h.w1 = (float)(1.0 - beta1);
   h.b2 = (float)beta2;
   h.omb2 = (float)(1.0 - beta2);
+  h.w1_lo = (float)((1.0 - beta1) - h.w1);
+  h.b2_lo = (float)(beta2 - h.b2);
+  h.omb2_lo = (float)((1.0 - beta2) - h.omb2);
   h.inv_bc2_sqrt = (float)(1.0 / std::sqrt(1.0 - std::pow(beta2, (double)step)));
   h.eps = (float)eps;
   h.neg_step = (float)(-(lr / (1.0 - std::pow(beta1, (double)step))));
