@@ -581,6 +581,86 @@ __global__ void __launch_bounds__(256) linear_join_kernel(const GemmArgs a) {
   }
 }
 
+// ------------------------------------------------------------------ fp32 as it lies
+// fp32 operands without the split: v_mfma_f32_32x32x2_f32 takes exact products at a sixteenth of the 16-bit rate (three
+// products of half the width each: a fifth as fast as the planes'), but reads what the caller holds, in one launch where
+// the planes and their powers of two take up to seven. 64 x 64 tiles of four waves, 32 k a step; the next step's values are fetched
+// into registers while this one's are multiplied out of the other half of LDS, where k is the row, so that both
+// forms are read at 32 neighbouring words.
+constexpr int kPlainTile = 64, kPlainK = 32;
+
+// eight values of a thread's row from k on: (row, k + j), zeros outside
+template <bool KC>
+__device__ __forceinline__ void plain_load(const float* p, long long ld, int row, int R, int k, int K, bool vec, float (&v)[8]) {
+  if constexpr (KC) {
+    const float* q = p + row * ld + k;
+    if (vec && row < R && k + 8 <= K) {
+      const f32x4 a = *reinterpret_cast<const f32x4*>(q), b = *reinterpret_cast<const f32x4*>(q + 4);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        v[j] = a[j];
+        v[4 + j] = b[j];
+      }
+    } else {
+#pragma unroll
+      for (int j = 0; j < 8; ++j) v[j] = row < R && k + j < K ? q[j] : 0.f;
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = row < R && k + j < K ? p[(k + j) * ld + row] : 0.f;
+  }
+}
+
+template <bool AKC, bool BKC>
+__global__ void __launch_bounds__(256) linear_plain_kernel(const GemmArgs a, bool avec, bool bvec) {
+  __shared__ float sA[2][kPlainK][kPlainTile], sB[2][kPlainK][kPlainTile];
+  const int NT = (a.N + kPlainTile - 1) / kPlainTile;
+  const int m0 = blockIdx.x / NT * kPlainTile, n0 = blockIdx.x % NT * kPlainTile;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int wm = (wave >> 1) * 32, wn = (wave & 1) * 32, r = lane & 31, half = lane >> 5;
+  const float* A = reinterpret_cast<const float*>(a.A);
+  const float* B = reinterpret_cast<const float*>(a.B);
+  const int s0 = blockIdx.y * a.per, s1 = min(a.steps, s0 + a.per);
+  f32x16 acc = {};
+  float va[8], vb[8];
+  auto fetch = [&](int s) __attribute__((always_inline)) {
+    const int k = s * kPlainK + wave * 8;
+    plain_load<AKC>(A, a.lda, m0 + lane, a.M, k, a.K, avec, va);
+    plain_load<BKC>(B, a.ldb, n0 + lane, a.N, k, a.K, bvec, vb);
+  };
+  fetch(s0);
+  for (int s = s0; s < s1; ++s) {
+    const int b = (s - s0) & 1;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      sA[b][wave * 8 + j][lane] = va[j];
+      sB[b][wave * 8 + j][lane] = vb[j];
+    }
+    __syncthreads();   // the half written before last is read by nobody any more
+    if (s + 1 < s1) fetch(s + 1);
+#pragma unroll
+    for (int k = 0; k < kPlainK; k += 2)
+      acc = __builtin_amdgcn_mfma_f32_32x32x2f32(sA[b][k + half][wm + r], sB[b][k + half][wn + r], acc, 0, 0, 0);
+  }
+  const int n = n0 + wn + r;
+  if (n >= a.N) return;
+  float* slab = a.splits > 1 ? a.slab + (long long)blockIdx.y * a.M * a.N : nullptr;
+  Cols<float, 1> cols;
+  if (!slab) cols.load(a.e, n);
+#pragma unroll
+  for (int i = 0; i < 16; ++i) {
+    const long long m = m0 + wm + (i >> 2) * 8 + half * 4 + (i & 3);
+    if (m >= a.M) continue;
+    if (slab) {
+      slab[m * a.N + n] = acc[i];
+    } else {
+      float v[1] = {acc[i]}, res[1] = {0.f};
+      if (a.e.res) res[0] = static_cast<const float*>(a.e.res)[m * a.e.ldr + n];
+      epilogue<float, 1, true>(a.e, cols, m, n, v, res, 0);
+    }
+  }
+}
+
 // ------------------------------------------------------------------ few rows
 // Up to 64 rows of x: bound by the one read of W. A workgroup takes 16 rows of W (columns of y), its waves a slice of K each;
 // a lane fetches 16 bytes of its row of W and of its rows of x straight into the fragments of v_mfma_f32_16x16x32 (fp32: four
@@ -891,6 +971,7 @@ inline unsigned blocks_for(long long n) { return (unsigned)std::min<long long>((
 struct Shape {
   int tile, per;
   long long tiles;
+  double us;
 };
 inline Shape shape_of(int M, int N, int steps, double products) {   // products: of a step, against 16 bits
   Shape best{};
@@ -910,8 +991,31 @@ inline Shape shape_of(int M, int N, int steps, double products) {   // products:
       if (splits > 1) us += 3 + (double)M * N * (6.0 * splits + 2) / 4.5e6;
       if (us < least) {
         least = us;
-        best = Shape{t, per, tiles};
+        best = Shape{t, per, tiles, us};
       }
+    }
+  }
+  return best;
+}
+
+// The same for fp32 operands as they lie, 64 x 64 tiles and 32 k a step: four workgroups a CU take 2.6 us a step, 0.5 more for
+// each operand read across its rows and 1.4 for rows off 16 bytes, two and one a CU 0.55 and 0.4 of it. Measured on
+// 17 sizes in each direction, laid-out planes against this: 1365 x 83 x 76: 17, 22 and 28 us against 9, 9 and 10;
+// 1000^3: 36, 40 and 44 against 35, 38 and 39; 2048 x 1024 x 1024: 43, 47 and 55 against 47, 59 and 65.
+inline Shape plain_shape_of(int M, int N, int steps, double each) {
+  Shape best{};
+  double least = 1e300;
+  const long long tiles = (long long)((M + kPlainTile - 1) / kPlainTile) * ((N + kPlainTile - 1) / kPlainTile);
+  for (int p = 1; p <= 64; p = p < 8 ? p + 1 : p + p / 4) {
+    const int per = (steps + p - 1) / p, splits = (steps + per - 1) / per;
+    if (p > 1 && (per < 2 || splits < 2)) break;
+    const long long blocks = tiles * splits, slots = 1024, rounds = blocks / slots, rest = blocks - rounds * slots;
+    const double last = rest == 0 ? 0 : 3 + per * (rest <= 256 ? 0.4 : rest <= 512 ? 0.55 : 1) * each;
+    double us = rounds * (4.5 + each * per) + last;
+    if (splits > 1) us += 4 + (double)M * N * (6.0 * splits + 2) / 4.5e6;
+    if (us < least) {
+      least = us;
+      best = Shape{kPlainTile, per, tiles, us};
     }
   }
   return best;
@@ -987,6 +1091,32 @@ struct Pass {
     else
       hipLaunchKernelGGL((linear_gemm_kernel<H, S, AKC, BKC, RES, 128, 128, 2, 2>), grid, dim3(256), 0, st, a);
   }
+  // fp32: multiplies the operands as they lie where that is estimated to be faster than laying planes out for it
+  template <bool AKC, bool BKC>
+  bool plain(const void* A, long long lda, const void* B, long long ldb, int M, int N, int K, const Epi& e) {
+    GemmArgs a{};
+    a.M = M; a.N = N; a.K = K;
+    a.A = static_cast<const u16*>(A); a.B = static_cast<const u16*>(B);
+    a.lda = lda; a.ldb = ldb;
+    a.e = e;
+    a.steps = (K + kPlainK - 1) / kPlainK;
+    const bool avec = lda % 4 == 0 && ((uintptr_t)A & 15) == 0, bvec = ldb % 4 == 0 && ((uintptr_t)B & 15) == 0;
+    auto slow = [](bool kc, bool vec) { return kc ? (vec ? 0 : 1.4) : 0.5; };
+    const Shape c = plain_shape_of(M, N, a.steps, 2.6 + slow(AKC, avec) + slow(BKC, bvec));
+    // planes: a launch and one pass over an operand by rows, three and two by columns
+    auto laid = [](bool kc, double n) { return kc ? 5 + n * 8 / 4.5e6 : 14 + n * 12 / 4.5e6; };
+    const double planes = shape_of(M, N, (2 * ((K + 31) / 32 * 32) + kBK - 1) / kBK, 1.5).us +
+                          laid(AKC, (double)M * K) + laid(BKC, (double)N * K);
+    if (c.us > planes || c.tiles > 0xffffff) return false;
+    a.per = c.per;
+    a.splits = (a.steps + a.per - 1) / a.per;
+    if (a.splits > 1) a.slab = ws.take<float>((long long)a.splits * M * N);
+    if (!run || rc != SE_OK) return true;
+    hipLaunchKernelGGL((linear_plain_kernel<AKC, BKC>), dim3((unsigned)c.tiles, a.splits), dim3(256), 0, st, a, avec, bvec);
+    launched();
+    if (a.splits > 1) join<float>(a);
+    return true;
+  }
   template <typename H, typename S, bool AKC, bool BKC>
   void product(const Mat& A, const Mat& B, int M, int N, int K, const Epi& e) {
     GemmArgs a{};
@@ -1011,18 +1141,22 @@ struct Pass {
       start<H, S, AKC, BKC, false>(a, c);
     }
     launched();
-    if (a.splits > 1) {
-      // 4 columns a thread where the rows of everything are aligned for it
-      auto ok = [&](int v) {
-        const uintptr_t al = std::min<int>(16, v * sizeof(S)) - 1;
-        return N % v == 0 && (((uintptr_t)e.C | (uintptr_t)e.bias | (uintptr_t)e.res) & al) == 0 && e.ldc % v == 0 &&
-               (!e.res || e.ldr % v == 0);
-      };
-      const long long mn = (long long)M * N;
-      if (ok(4)) hipLaunchKernelGGL((linear_join_kernel<S, 4>), dim3(blocks_for(mn / 4)), dim3(256), 0, st, a);
-      else hipLaunchKernelGGL((linear_join_kernel<S, 1>), dim3(blocks_for(mn)), dim3(256), 0, st, a);
-      launched();
-    }
+    if (a.splits > 1) join<S>(a);
+  }
+  template <typename S>
+  void join(const GemmArgs& a) {
+    const Epi& e = a.e;
+    const int N = a.N;
+    // 4 columns a thread where the rows of everything are aligned for it
+    auto ok = [&](int v) {
+      const uintptr_t al = std::min<int>(16, v * sizeof(S)) - 1;
+      return N % v == 0 && (((uintptr_t)e.C | (uintptr_t)e.bias | (uintptr_t)e.res) & al) == 0 && e.ldc % v == 0 &&
+             (!e.res || e.ldr % v == 0);
+    };
+    const long long mn = (long long)a.M * N;
+    if (ok(4)) hipLaunchKernelGGL((linear_join_kernel<S, 4>), dim3(blocks_for(mn / 4)), dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((linear_join_kernel<S, 1>), dim3(blocks_for(mn)), dim3(256), 0, st, a);
+    launched();
   }
 };
 
@@ -1062,6 +1196,8 @@ int forward(const se_linear_desc* d, const void* x, const void* w, const void* b
     p.launched();
     return p.rc;
   }
+  if constexpr (f32)
+    if (p.template plain<true, true>(x, d->ldx, w, d->ldw, d->M, d->N, d->K, e)) return p.rc;
   const Mat A = f32 ? p.planes(x, d->ldx, d->M, d->K, true) : p.half(x, d->ldx, d->M, d->K);
   const Mat B = f32 ? p.planes(w, d->ldw, d->N, d->K, true) : p.half(w, d->ldw, d->N, d->K);
   p.template product<H, S, true, true>(A, B, d->M, d->N, d->K, e);
@@ -1106,18 +1242,26 @@ int backward(const se_linear_desc* d, const void* dy, const void* x, const void*
   const void* gp = as_is ? dy : g;
   const long long ldg = as_is ? d->ldr : Np;
   if (dx) {
-    const Mat A = f32 ? p.planes(gp, ldg, M, N, true) : p.half(gp, ldg, M, as_is ? N : Np);
-    const Mat B = f32 ? p.planes(w, d->ldw, N, K, false) : p.half(w, d->ldw, N, K);
     Epi e{};
     e.C = dx; e.ldc = K;
-    p.template product<H, S, true, false>(A, B, M, K, N, e);
+    bool done = false;
+    if constexpr (f32) done = p.template plain<true, false>(gp, ldg, w, d->ldw, M, K, N, e);
+    if (!done) {
+      const Mat A = f32 ? p.planes(gp, ldg, M, N, true) : p.half(gp, ldg, M, as_is ? N : Np);
+      const Mat B = f32 ? p.planes(w, d->ldw, N, K, false) : p.half(w, d->ldw, N, K);
+      p.template product<H, S, true, false>(A, B, M, K, N, e);
+    }
   }
   if (dw) {
-    const Mat A = f32 ? p.planes(gp, ldg, M, N, false) : p.half(gp, ldg, M, as_is ? N : Np);
-    const Mat B = f32 ? p.planes(x, d->ldx, M, K, false) : p.half(x, d->ldx, M, K);
     Epi e{};
     e.C = dw; e.ldc = K;
-    p.template product<H, S, false, false>(A, B, N, K, M, e);
+    bool done = false;
+    if constexpr (f32) done = p.template plain<false, false>(gp, ldg, x, d->ldx, N, K, M, e);
+    if (!done) {
+      const Mat A = f32 ? p.planes(gp, ldg, M, N, false) : p.half(gp, ldg, M, as_is ? N : Np);
+      const Mat B = f32 ? p.planes(x, d->ldx, M, K, false) : p.half(x, d->ldx, M, K);
+      p.template product<H, S, false, false>(A, B, N, K, M, e);
+    }
   }
   return p.rc;
 }

@@ -62,10 +62,12 @@ def test_linear_c_arguments():
     assert fwd(D(3, 4, 8, 0, 1, 4, 8, 4)) == -1        # rows of x would overlap
     assert fwd(D(3, 4, 8, 0, 1, 8, 4, 4)) == -1        # rows of W would
     assert fwd(D(3, 4, 1 << 22, 0, 1, 1 << 22, 1 << 22, 4)) == -3
-    d = D(70, 4, 8, 0, 0, 8, 8, 4)
+    d = D(2500, 1030, 1030, 0, 0, 1030, 1030, 1030)
     need = lib.se_linear_fwd_workspace_size(ctypes.byref(d), p, p)
     assert need > 0                                     # fp32: the planes
     assert fwd(d, need - 1) == -5
+    # a small product multiplies fp32 as it lies
+    assert lib.se_linear_fwd_workspace_size(ctypes.byref(D(70, 4, 8, 0, 0, 8, 8, 4)), p, p) == 0
     assert lib.se_linear_fwd_workspace_size(ctypes.byref(D(0, 4, 8, 0, 0, 8, 8, 4)), p, p) == 0
     # bf16 on 16 bytes reads x and W as they lie; a row off 16 bytes is packed
     assert lib.se_linear_fwd_workspace_size(ctypes.byref(D(70, 4, 8, 0, 1, 8, 8, 4)), p, p) == 0

@@ -8,12 +8,14 @@ Bounds, u = 2^-24, e = eps(type) / 2, S = sum_k |x w| (+ |b|):
   functions are a few u off.
   g = dy act'(z~), z~ the stored z: off by the slope's range over z (1 +- e) +- D, and rounded once more (e) in 16 bits;
   then dx, dW, db are sums of such terms, each with its own accumulation error, rounded once."""
+import ctypes
 import math
 
 import pytest
 import torch
 import torch.nn as nn
 
+from sehip import _native as N
 from sehip import linear
 
 pytestmark = pytest.mark.gpu
@@ -335,3 +337,58 @@ def test_refusals_on_the_gpu(gpu_device):
     (dx,) = torch.autograd.grad(y.square().sum(), x, create_graph=True)
     with pytest.raises(RuntimeError):   # once differentiable
         dx.sum().backward()
+
+
+# ------------------------------------------------------------------ fp32 in both its forms
+# Small products multiply fp32 as it lies, large ones the hi and lo halves of a laid-out copy: sizes of either side of the rule.
+FORMS = [(2500, 1030, 1030), (1500, 2050, 1026), (700, 1030, 130)]
+
+
+@pytest.mark.parametrize("m,k,n", FORMS)
+@pytest.mark.parametrize("act", ("none", "silu"))
+def test_fp32_forms(gpu_device, m, k, n, act):
+    x, lin, res, dy = _make(gpu_device, torch.float32, m, k, n, seed=11)
+    d = N.LinearDesc(m, n, k, 0, 0, k, k, n)
+    need = N.lib().se_linear_fwd_workspace_size(ctypes.byref(d), ctypes.c_void_p(256), ctypes.c_void_p(256))
+    # as it lies: no workspace, or a slab of sums for each part of a split K and nothing else
+    slabs = {-(-4 * parts * m * n // 256) * 256 for parts in (0, *range(2, 65))}
+    assert (need in slabs) == (m < 1000)
+    y, grads = _run(x, lin, act, res, dy)
+    _check(x, lin.weight, lin.bias, res, act, dy, y, grads)
+    again = _run(x, lin, act, res, dy)
+    assert torch.equal(y, again[0]) and all(torch.equal(a, b) for a, b in zip(grads, again[1]))
+
+
+@pytest.mark.parametrize("m,k,n", FORMS)
+def test_fp32_forms_keep_rows_apart(gpu_device, m, k, n):
+    """As the two tests above it of small sizes: what is not finite stays in its row, quiet rows and columns keep their digits."""
+    x, lin, _, dy = _make(gpu_device, torch.float32, m, k, n, residual=False, seed=12)
+    x[1::2] *= 2.0 ** -30
+    with torch.no_grad():
+        lin.weight[::3] *= 2.0 ** -20
+        lin.bias.zero_()
+    dy[:, ::5] *= 2.0 ** -24
+    y, grads = _run(x, lin, "none", None, dy)
+    _check(x, lin.weight, lin.bias, None, "none", dy, y, grads)
+    x[5, 3], x[77, k - 1], x[m - 1, 0] = float("nan"), float("inf"), float("-inf")
+    dy[9, 1] = float("inf")
+    z, bad = _run(x, lin, "none", None, dy)
+    keep = torch.ones(m, dtype=torch.bool, device=gpu_device)
+    keep[[5, 77, m - 1]] = False
+    assert torch.equal(z[keep], y[keep]) and not z[[5, m - 1]].isfinite().all(1).any() and not z[77].isfinite().all()
+    keep[:] = True
+    keep[9] = False
+    assert torch.equal(bad[0][keep], grads[0][keep]) and not bad[0][9].isfinite().all()
+
+
+def test_fp32_as_it_lies_off_16_bytes(gpu_device):
+    """Rows, columns and starts off the vector loads' alignment, odd sizes, K in the last eight of a step."""
+    torch.manual_seed(13)
+    base = torch.randn(90, 140, device=gpu_device)
+    for k in (31, 32, 33, 39, 40, 41, 63, 65):
+        for off in (0, 1, 4):
+            x = base[:, off:off + k]
+            lin = nn.Linear(k, 67, device=gpu_device)
+            dy = torch.randn(90, 67, device=gpu_device)
+            y, grads = _run(x, lin, "gelu", None, dy)
+            _check(x, lin.weight, lin.bias, None, "gelu", dy, y, grads)
