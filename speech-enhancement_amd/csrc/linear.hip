@@ -12,7 +12,7 @@
 // ds_read_b64_tr_b16, which hands every lane four consecutive k of its own row. A direct load leaves lane l's
 // 16 bytes at l * 16, so the image is swizzled on the side of memory: which chunk of its row a lane fetches.
 //
-// fp32 storage: each operand is split beforehand into fp16 x 2^(14 - e) = hi + lo (22 significant bits), e from the
+// fp32 storage, but for small products (linear_plain_kernel): each operand is split beforehand into fp16 x 2^(14 - e) = hi + lo (22 significant bits), e from the
 // largest magnitude of its own free index (a row of x has its own scale, so a loud frame costs a quiet one no digits, and
 // an infinity stays in its row). 32 k of hi and the same 32 of lo lie side by side, 64 k of a tile, whose products are hi hi,
 // hi lo and lo hi; the epilogue multiplies by 2^(ea + eb - 28).
@@ -582,9 +582,9 @@ __global__ void __launch_bounds__(256) linear_join_kernel(const GemmArgs a) {
 }
 
 // ------------------------------------------------------------------ fp32 as it lies
-// fp32 operands without the split: v_mfma_f32_32x32x2_f32 takes exact products at a sixteenth of the 16-bit rate (three
-// products of half the width each: a fifth as fast as the planes'), but reads what the caller holds, in one launch where
-// the planes and their powers of two take up to seven. 64 x 64 tiles of four waves, 32 k a step; the next step's values are fetched
+// fp32 operands without the split: v_mfma_f32_32x32x2_f32 multiplies at a sixteenth of the 16-bit rate, a fifth of what the
+// planes' three products reach, but reads what the caller holds, in one launch where the planes and their powers of
+// two take up to seven: for small products, by the rule at plain_shape_of. 64 x 64 tiles of four waves, 32 k a step; the next step's values are fetched
 // into registers while this one's are multiplied out of the other half of LDS, where k is the row, so that both
 // forms are read at 32 neighbouring words.
 constexpr int kPlainTile = 64, kPlainK = 32;
