@@ -773,10 +773,9 @@ __device__ __forceinline__ void split(float x, int e, _Float16& hi, _Float16& lo
 // fp32 [R][C] at ld -> rows of 64 to each 32 columns (hi, then lo; zeros behind C), one power of two a row. A wave takes a row, a lane
 // pairs of columns; rows of up to 2048 stay in registers, longer ones are read again.
 constexpr int kSplitKeep = 16;
-template <bool TWO>
-__device__ __forceinline__ void load_two(const float* p, int c, int C, float& a, float& b) {
+__device__ __forceinline__ void load_two(bool two, const float* p, int c, int C, float& a, float& b) {
   a = b = 0.f;
-  if (TWO && c + 1 < C) {
+  if (two && c + 1 < C) {
     const float2 t = *reinterpret_cast<const float2*>(p + c);
     a = t.x;
     b = t.y;
@@ -793,10 +792,29 @@ __device__ __forceinline__ void split_two(float a, float b, int ea, int eb, unsi
   hi = __builtin_bit_cast(unsigned, (f16x2){h0, h1});
   lo = __builtin_bit_cast(unsigned, (f16x2){l0, l1});
 }
-template <bool TWO>
-__global__ void __launch_bounds__(256) linear_split_rows_kernel(const float* __restrict__ x, long long ld, int R, int C,
-                                                                int C32, unsigned* __restrict__ out,
-                                                                short* __restrict__ ex) {
+// An operand to be laid out. A launch takes the operands of a pass side by side (blockIdx.z), since alone the small ones
+// take what a launch takes.
+struct SplitJob {
+  const float* x;   // [R][C] at ld
+  long long ld;
+  unsigned* out;
+  short* ex;        // the powers of two
+  float* part;      // by columns: [parts][C] largest magnitudes of chunks of `rows` rows
+  int R, C, width;  // width: C32 (by rows) or Cp (by columns)
+  int rows, parts;
+  bool two, known;  // two: pairs are aligned; known: `part` is there
+};
+constexpr int kMostJobs = 3;
+struct SplitJobs {
+  SplitJob j[kMostJobs];
+};
+__global__ void __launch_bounds__(256) linear_split_rows_kernel(const SplitJobs jobs) {
+  const SplitJob& t = jobs.j[blockIdx.z];
+  const float* __restrict__ x = t.x;
+  unsigned* __restrict__ out = t.out;
+  const long long ld = t.ld;
+  const int R = t.R, C = t.C, C32 = t.width;
+  const bool two = t.two;
   const int lane = threadIdx.x & 63;
   for (long long r = blockIdx.x * 4LL + (threadIdx.x >> 6); r < R; r += gridDim.x * 4LL) {
     const float* p = x + r * ld;
@@ -805,16 +823,16 @@ __global__ void __launch_bounds__(256) linear_split_rows_kernel(const float* __r
 #pragma unroll
     for (int i = 0; i < kSplitKeep; ++i) {
       v[i][0] = v[i][1] = 0.f;
-      if (i * 128 < C) load_two<TWO>(p, i * 128 + 2 * lane, C, v[i][0], v[i][1]);
+      if (i * 128 < C) load_two(two, p, i * 128 + 2 * lane, C, v[i][0], v[i][1]);
       m = fmaxf(m, fmaxf(finite_abs(v[i][0]), finite_abs(v[i][1])));
     }
     for (int c = kSplitKeep * 128 + 2 * lane; c < C; c += 128) {
       float a, b;
-      load_two<TWO>(p, c, C, a, b);
+      load_two(two, p, c, C, a, b);
       m = fmaxf(m, fmaxf(finite_abs(a), finite_abs(b)));
     }
     const int e = exp_of(se::wave_max(m));
-    if (lane == 0) ex[r] = (short)e;
+    if (lane == 0) t.ex[r] = (short)e;
     auto put = [&](int c, float a, float b) __attribute__((always_inline)) {
       unsigned hi, lo;
       split_two(a, b, e, e, hi, lo);
@@ -827,7 +845,7 @@ __global__ void __launch_bounds__(256) linear_split_rows_kernel(const float* __r
       if (i * 128 + 2 * lane < C32) put(i * 128 + 2 * lane, v[i][0], v[i][1]);
     for (int c = kSplitKeep * 128 + 2 * lane; c < C32; c += 128) {
       float a, b;
-      load_two<TWO>(p, c, C, a, b);
+      load_two(two, p, c, C, a, b);
       put(c, a, b);
     }
   }
@@ -835,40 +853,43 @@ __global__ void __launch_bounds__(256) linear_split_rows_kernel(const float* __r
 
 // the same with one power of two a column, 32 rows of hi, then the 32 of lo: the columns' largest magnitudes over chunks
 // of rows, their powers, then the halves in rows of Cp
-__global__ void __launch_bounds__(256) linear_col_max_kernel(const float* __restrict__ x, long long ld, int R, int C,
-                                                             int rows, float* __restrict__ part) {
+__global__ void __launch_bounds__(256) linear_col_max_kernel(const SplitJobs jobs) {
+  const SplitJob& t = jobs.j[blockIdx.z];
   const int c = blockIdx.x * 256 + threadIdx.x;
-  if (c >= C) return;
-  const int r0 = blockIdx.y * rows, r1 = min(R, r0 + rows);
+  if (c >= t.C || (int)blockIdx.y >= t.parts || t.known) return;
+  const float* __restrict__ x = t.x + c;
+  const int r0 = blockIdx.y * t.rows, r1 = min(t.R, r0 + t.rows);
   float m = 0.f;
 #pragma unroll 8
-  for (int r = r0; r < r1; ++r) m = fmaxf(m, finite_abs(x[r * ld + c]));
-  part[(long long)blockIdx.y * C + c] = m;
+  for (int r = r0; r < r1; ++r) m = fmaxf(m, finite_abs(x[r * t.ld]));
+  t.part[(long long)blockIdx.y * t.C + c] = m;
 }
-__global__ void __launch_bounds__(1024) linear_col_exp_kernel(const float* __restrict__ part, int parts, int C,
-                                                              short* __restrict__ ex) {
+__global__ void __launch_bounds__(1024) linear_col_exp_kernel(const SplitJobs jobs) {
   __shared__ float s[16][64];
+  const SplitJob& t = jobs.j[blockIdx.z];
   const int l = threadIdx.x & 63, k = threadIdx.x >> 6, c = blockIdx.x * 64 + l;
   float m = 0.f;
-  if (c < C)
+  if (c < t.C)
 #pragma unroll 8
-    for (int i = k; i < parts; i += 16) m = fmaxf(m, part[(long long)i * C + c]);
+    for (int i = k; i < t.parts; i += 16) m = fmaxf(m, t.part[(long long)i * t.C + c]);
   s[k][l] = m;
   __syncthreads();
-  if (k || c >= C) return;
+  if (k || c >= t.C) return;
   for (int i = 1; i < 16; ++i) m = fmaxf(m, s[i][l]);
-  ex[c] = (short)exp_of(m);
+  t.ex[c] = (short)exp_of(m);
 }
-template <bool TWO>
-__global__ void __launch_bounds__(256) linear_split_cols_kernel(const float* __restrict__ x, long long ld, int R, int R32, int C,
-                                                                int Cp, const short* __restrict__ ex,
-                                                                unsigned* __restrict__ out) {
-  const int per = Cp / 2;
-  const long long total = (long long)R32 * per;
+__global__ void __launch_bounds__(256) linear_split_cols_kernel(const SplitJobs jobs) {
+  const SplitJob& t = jobs.j[blockIdx.z];
+  const float* __restrict__ x = t.x;
+  const short* __restrict__ ex = t.ex;
+  unsigned* __restrict__ out = t.out;
+  const int per = t.width / 2, R = t.R, C = t.C;
+  const bool two = t.two;
+  const long long total = (R + 31LL) / 32 * 32 * per;
   for (long long i = blockIdx.x * 256LL + threadIdx.x; i < total; i += gridDim.x * 256LL) {
     const int r = (int)(i / per), c = (int)(i - (long long)r * per) * 2;
     float a = 0.f, b = 0.f;
-    if (r < R) load_two<TWO>(x + r * ld, c, C, a, b);
+    if (r < R) load_two(two, x + r * t.ld, c, C, a, b);
     unsigned hi, lo;
     split_two(a, b, c < C ? ex[c] : 0, c + 1 < C ? ex[c + 1] : 0, hi, lo);
     const long long at = ((long long)(r >> 5) * 64 + (r & 31)) * per + c / 2;
@@ -879,19 +900,22 @@ __global__ void __launch_bounds__(256) linear_split_cols_kernel(const float* __r
 
 // g = dy act'(z) in rows of Np (zeros behind N), and each chunk of rows' column sums of g. z NULL: g = dy; g NULL: the
 // sums alone. A lane takes eight columns, cg lanes (a power of two) a row, 256 / cg rows at a time; the block's sums
-// of a column are added in a fixed order through LDS. Bound by memory: 16384 x 8192 bf16 in 163 us, 4.9 TB/s, 190 behind
+// of a column are added in a fixed order through LDS; top (fp32, or NULL): and their largest finite magnitudes, for the
+// powers of two of g's columns. Bound by memory: 16384 x 8192 bf16 in 163 us, 4.9 TB/s, 190 behind
 // large products (a column a lane: 367).
 template <typename S, bool VEC>
 __global__ void __launch_bounds__(256) linear_slope_kernel(const S* __restrict__ dy, long long ld, const S* __restrict__ z,
                                                            int act, int M, int N, int Np, int cg, int rows,
-                                                           S* __restrict__ g, float* __restrict__ part) {
+                                                           S* __restrict__ g, float* __restrict__ part,
+                                                           float* __restrict__ top) {
   __shared__ float sum[256][9];
   const int c = threadIdx.x % cg, n = (blockIdx.x * cg + c) * 8, step = 256 / cg;
   const long long r0 = (long long)blockIdx.y * rows;
   const int r1 = (int)min((long long)M - r0, (long long)rows);
-  float s[8];
+  constexpr bool f32 = sizeof(S) == 4;
+  float s[8], t8[8];
 #pragma unroll
-  for (int j = 0; j < 8; ++j) s[j] = 0.f;
+  for (int j = 0; j < 8; ++j) s[j] = t8[j] = 0.f;
   if (n < Np)
 #pragma unroll 2
     for (int r = threadIdx.x / cg; r < r1; r += step) {
@@ -913,17 +937,35 @@ __global__ void __launch_bounds__(256) linear_slope_kernel(const S* __restrict__
       if (g) store_pack<S, 8>(g + m * Np + n, v);
 #pragma unroll
       for (int j = 0; j < 8; ++j) s[j] += v[j];
-    }
-  if (!part) return;
+      if constexpr (f32)
 #pragma unroll
-  for (int j = 0; j < 8; ++j) sum[threadIdx.x][j] = s[j];
-  __syncthreads();
-  for (int i = threadIdx.x; i < cg * 8; i += 256) {
-    const int at = blockIdx.x * cg * 8 + i;
-    if (at >= N) continue;
-    float v = 0.f;
-    for (int k = 0; k < step; ++k) v += sum[k * cg + i / 8][i & 7];
-    part[(long long)blockIdx.y * N + at] = v;
+        for (int j = 0; j < 8; ++j) t8[j] = fmaxf(t8[j], finite_abs(v[j]));
+    }
+  if (part) {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) sum[threadIdx.x][j] = s[j];
+    __syncthreads();
+    for (int i = threadIdx.x; i < cg * 8; i += 256) {
+      const int at = blockIdx.x * cg * 8 + i;
+      if (at >= N) continue;
+      float v = 0.f;
+      for (int k = 0; k < step; ++k) v += sum[k * cg + i / 8][i & 7];
+      part[(long long)blockIdx.y * N + at] = v;
+    }
+  }
+  if constexpr (f32) {
+    if (!top) return;
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < 8; ++j) sum[threadIdx.x][j] = t8[j];
+    __syncthreads();
+    for (int i = threadIdx.x; i < cg * 8; i += 256) {
+      const int at = blockIdx.x * cg * 8 + i;
+      if (at >= N) continue;
+      float v = 0.f;
+      for (int k = 0; k < step; ++k) v = fmaxf(v, sum[k * cg + i / 8][i & 7]);
+      top[(long long)blockIdx.y * N + at] = v;
+    }
   }
 }
 
@@ -1052,35 +1094,57 @@ struct Pass {
     m.bytes = (long long)R * Cp * 2;
     return m;
   }
-  // fp32 [R][C] at ld as hi and lo, powers of two by row (reduced along the row) or by column (along the column)
-  Mat planes(const void* xv, long long ld, int R, int C, bool by_row) {
-    const float* x = static_cast<const float*>(xv);
-    const bool two = ld % 2 == 0 && ((uintptr_t)x & 7) == 0;
-    const int C32 = (C + 31) / 32 * 32, R32 = (R + 31) / 32 * 32, Cp = up8(C);
+  // fp32 [R][C] at ld as hi and lo, powers of two by row (reduced along the row) or by column (along the column); what is
+  // registered is laid out by lay(). top: the columns' largest magnitudes over `parts` chunks of rows, if they are known
+  SplitJobs by_rows{}, by_cols{};
+  int n_rows = 0, n_cols = 0;
+  Mat planes(const void* xv, long long ld, int R, int C, bool by_row, float* top = nullptr, int parts = 0) {
+    SplitJob t{};
+    t.x = static_cast<const float*>(xv);
+    t.ld = ld;
+    t.R = R; t.C = C;
+    t.width = by_row ? (C + 31) / 32 * 32 : up8(C);
+    t.two = ld % 2 == 0 && ((uintptr_t)xv & 7) == 0;
     Mat m{};
-    m.ld = by_row ? 2LL * C32 : Cp;
-    m.bytes = (by_row ? (long long)R : 2LL * R32) * m.ld * 2;
+    m.ld = by_row ? 2LL * t.width : t.width;
+    m.bytes = (by_row ? (long long)R : 2LL * ((R + 31) / 32 * 32)) * m.ld * 2;
     u16* out = ws.take<u16>(m.bytes / 2);
-    short* ex = ws.take<short>(by_row ? R : C);
     m.p = out;
-    m.ex = ex;
-    const int rows = std::max(64, (R + 255) / 256), parts = (R + rows - 1) / rows;
-    float* part = by_row ? nullptr : ws.take<float>((long long)parts * C);
-    if (!run) return m;
-    unsigned* to = reinterpret_cast<unsigned*>(out);
-    if (by_row) {
-      const dim3 grid((unsigned)std::min<long long>((R + 3LL) / 4, 1 << 20));
-      if (two) hipLaunchKernelGGL(linear_split_rows_kernel<true>, grid, dim3(256), 0, st, x, ld, R, C, C32, to, ex);
-      else hipLaunchKernelGGL(linear_split_rows_kernel<false>, grid, dim3(256), 0, st, x, ld, R, C, C32, to, ex);
-    } else {
-      hipLaunchKernelGGL(linear_col_max_kernel, dim3((C + 255) / 256, parts), dim3(256), 0, st, x, ld, R, C, rows, part);
-      hipLaunchKernelGGL(linear_col_exp_kernel, dim3((C + 63) / 64), dim3(1024), 0, st, part, parts, C, ex);
-      const dim3 grid(blocks_for((long long)R32 * Cp / 2));
-      if (two) hipLaunchKernelGGL(linear_split_cols_kernel<true>, grid, dim3(256), 0, st, x, ld, R, R32, C, Cp, ex, to);
-      else hipLaunchKernelGGL(linear_split_cols_kernel<false>, grid, dim3(256), 0, st, x, ld, R, R32, C, Cp, ex, to);
+    m.ex = t.ex = ws.take<short>(by_row ? R : C);
+    t.out = reinterpret_cast<unsigned*>(out);
+    if (!by_row) {
+      t.known = parts > 0;
+      t.rows = std::max(64, (R + 255) / 256);
+      t.parts = t.known ? parts : (R + t.rows - 1) / t.rows;
+      t.part = t.known ? top : ws.take<float>((long long)t.parts * C);
     }
-    launched();
+    if (by_row) by_rows.j[n_rows++] = t;
+    else by_cols.j[n_cols++] = t;
     return m;
+  }
+  void lay() {
+    if (!run || rc != SE_OK) return;
+    if (n_rows) {
+      long long most = 0;
+      for (int i = 0; i < n_rows; ++i) most = std::max(most, (by_rows.j[i].R + 3LL) / 4);
+      const dim3 grid((unsigned)std::min<long long>(most, 1 << 20), 1, n_rows);
+      hipLaunchKernelGGL(linear_split_rows_kernel, grid, dim3(256), 0, st, by_rows);
+    }
+    if (n_cols) {
+      int C = 0, parts = 0;
+      unsigned blocks = 0;
+      for (int i = 0; i < n_cols; ++i) {
+        const SplitJob& t = by_cols.j[i];
+        C = std::max(C, t.C);
+        if (!t.known) parts = std::max(parts, t.parts);
+        blocks = std::max(blocks, blocks_for((t.R + 31LL) / 32 * 32 * t.width / 2));
+      }
+      if (parts) hipLaunchKernelGGL(linear_col_max_kernel, dim3((C + 255) / 256, parts, n_cols), dim3(256), 0, st, by_cols);
+      hipLaunchKernelGGL(linear_col_exp_kernel, dim3((C + 63) / 64, 1, n_cols), dim3(1024), 0, st, by_cols);
+      hipLaunchKernelGGL(linear_split_cols_kernel, dim3(blocks, 1, n_cols), dim3(256), 0, st, by_cols);
+    }
+    n_rows = n_cols = 0;
+    launched();
   }
 
   template <typename H, typename S, bool AKC, bool BKC, bool RES>
@@ -1091,9 +1155,20 @@ struct Pass {
     else
       hipLaunchKernelGGL((linear_gemm_kernel<H, S, AKC, BKC, RES, 128, 128, 2, 2>), grid, dim3(256), 0, st, a);
   }
-  // fp32: multiplies the operands as they lie where that is estimated to be faster than laying planes out for it
+  // fp32: the operands as they lie, where that is estimated to be faster than laying planes out (tiles 0: it is not)
   template <bool AKC, bool BKC>
-  bool plain(const void* A, long long lda, const void* B, long long ldb, int M, int N, int K, const Epi& e) {
+  Shape plain_of(const void* A, long long lda, const void* B, long long ldb, int M, int N, int K) {
+    const bool avec = lda % 4 == 0 && ((uintptr_t)A & 15) == 0, bvec = ldb % 4 == 0 && ((uintptr_t)B & 15) == 0;
+    auto slow = [](bool kc, bool vec) { return kc ? (vec ? 0 : 1.4) : 0.5; };
+    const Shape c = plain_shape_of(M, N, (K + kPlainK - 1) / kPlainK, 2.6 + slow(AKC, avec) + slow(BKC, bvec));
+    // planes: a launch and one pass over an operand by rows, three and two by columns
+    auto laid = [](bool kc, double n) { return kc ? 5 + n * 8 / 4.5e6 : 14 + n * 12 / 4.5e6; };
+    const double planes = shape_of(M, N, (2 * ((K + 31) / 32 * 32) + kBK - 1) / kBK, 1.5).us +
+                          laid(AKC, (double)M * K) + laid(BKC, (double)N * K);
+    return c.us > planes || c.tiles > 0xffffff ? Shape{} : c;
+  }
+  template <bool AKC, bool BKC>
+  void plain(const void* A, long long lda, const void* B, long long ldb, int M, int N, int K, const Epi& e, const Shape& c) {
     GemmArgs a{};
     a.M = M; a.N = N; a.K = K;
     a.A = static_cast<const u16*>(A); a.B = static_cast<const u16*>(B);
@@ -1101,21 +1176,13 @@ struct Pass {
     a.e = e;
     a.steps = (K + kPlainK - 1) / kPlainK;
     const bool avec = lda % 4 == 0 && ((uintptr_t)A & 15) == 0, bvec = ldb % 4 == 0 && ((uintptr_t)B & 15) == 0;
-    auto slow = [](bool kc, bool vec) { return kc ? (vec ? 0 : 1.4) : 0.5; };
-    const Shape c = plain_shape_of(M, N, a.steps, 2.6 + slow(AKC, avec) + slow(BKC, bvec));
-    // planes: a launch and one pass over an operand by rows, three and two by columns
-    auto laid = [](bool kc, double n) { return kc ? 5 + n * 8 / 4.5e6 : 14 + n * 12 / 4.5e6; };
-    const double planes = shape_of(M, N, (2 * ((K + 31) / 32 * 32) + kBK - 1) / kBK, 1.5).us +
-                          laid(AKC, (double)M * K) + laid(BKC, (double)N * K);
-    if (c.us > planes || c.tiles > 0xffffff) return false;
     a.per = c.per;
     a.splits = (a.steps + a.per - 1) / a.per;
     if (a.splits > 1) a.slab = ws.take<float>((long long)a.splits * M * N);
-    if (!run || rc != SE_OK) return true;
+    if (!run || rc != SE_OK) return;
     hipLaunchKernelGGL((linear_plain_kernel<AKC, BKC>), dim3((unsigned)c.tiles, a.splits), dim3(256), 0, st, a, avec, bvec);
     launched();
     if (a.splits > 1) join<float>(a);
-    return true;
   }
   template <typename H, typename S, bool AKC, bool BKC>
   void product(const Mat& A, const Mat& B, int M, int N, int K, const Epi& e) {
@@ -1196,10 +1263,16 @@ int forward(const se_linear_desc* d, const void* x, const void* w, const void* b
     p.launched();
     return p.rc;
   }
-  if constexpr (f32)
-    if (p.template plain<true, true>(x, d->ldx, w, d->ldw, d->M, d->N, d->K, e)) return p.rc;
+  if constexpr (f32) {
+    const Shape c = p.template plain_of<true, true>(x, d->ldx, w, d->ldw, d->M, d->N, d->K);
+    if (c.tiles) {
+      p.template plain<true, true>(x, d->ldx, w, d->ldw, d->M, d->N, d->K, e, c);
+      return p.rc;
+    }
+  }
   const Mat A = f32 ? p.planes(x, d->ldx, d->M, d->K, true) : p.half(x, d->ldx, d->M, d->K);
   const Mat B = f32 ? p.planes(w, d->ldw, d->N, d->K, true) : p.half(w, d->ldw, d->N, d->K);
+  p.lay();
   p.template product<H, S, true, true>(A, B, d->M, d->N, d->K, e);
   return p.rc;
 }
@@ -1222,16 +1295,26 @@ int backward(const se_linear_desc* d, const void* dy, const void* x, const void*
   const long long chunks = std::max(1, std::min(512, 2048 / across));
   const int rows = (int)std::max<long long>(4 * turn, (M + chunks - 1) / chunks), parts = (M + rows - 1) / rows;
   float* part = db ? p.ws.template take<float>((long long)parts * N) : nullptr;
-  if (p.run && (part || g)) {
+  const void* gp = as_is ? dy : g;
+  const long long ldg = as_is ? d->ldr : Np;
+  Shape cx{}, cw{};
+  if constexpr (f32) {
+    if (dx) cx = p.template plain_of<true, false>(gp, ldg, w, d->ldw, M, K, N);
+    if (dw) cw = p.template plain_of<false, false>(gp, ldg, x, d->ldx, N, K, M);
+  }
+  // the pass over dy leaves the largest magnitudes of g's columns where dW's planes need them
+  const bool passes = db || (prod && !as_is), tops = f32 && dw && !cw.tiles && passes;
+  float* top = tops ? p.ws.template take<float>((long long)parts * N) : nullptr;
+  if (p.run && passes) {
     const bool vec = N % 8 == 0 && ((uintptr_t)dy & 15) == 0 && d->ldr % (16 / sizeof(S)) == 0;
     const S* zs = sloped ? static_cast<const S*>(z) : nullptr;
     const S* dys = static_cast<const S*>(dy);
     if (vec)
       hipLaunchKernelGGL((linear_slope_kernel<S, true>), dim3(across, parts), dim3(256), 0, p.st, dys, d->ldr, zs, d->act,
-                         M, N, Np, cg, rows, g, part);
+                         M, N, Np, cg, rows, g, part, top);
     else
       hipLaunchKernelGGL((linear_slope_kernel<S, false>), dim3(across, parts), dim3(256), 0, p.st, dys, d->ldr, zs, d->act,
-                         M, N, Np, cg, rows, g, part);
+                         M, N, Np, cg, rows, g, part, top);
     p.launched();
     if (part) {
       hipLaunchKernelGGL(linear_bias_kernel<S>, dim3((N + 63) / 64), dim3(1024), 0, p.st, part, parts, N,
@@ -1239,29 +1322,28 @@ int backward(const se_linear_desc* d, const void* dy, const void* x, const void*
       p.launched();
     }
   }
-  const void* gp = as_is ? dy : g;
-  const long long ldg = as_is ? d->ldr : Np;
+  Epi ex{}, ew{};
+  ex.C = dx; ex.ldc = K;
+  ew.C = dw; ew.ldc = K;
+  Mat A{}, B{}, Aw{}, Bw{};
+  if (dx && !cx.tiles) {
+    A = f32 ? p.planes(gp, ldg, M, N, true) : p.half(gp, ldg, M, as_is ? N : Np);
+    B = f32 ? p.planes(w, d->ldw, N, K, false) : p.half(w, d->ldw, N, K);
+  }
+  if (dw && !cw.tiles) {
+    Aw = f32 ? p.planes(gp, ldg, M, N, false, top, tops ? parts : 0) : p.half(gp, ldg, M, as_is ? N : Np);
+    Bw = f32 ? p.planes(x, d->ldx, M, K, false) : p.half(x, d->ldx, M, K);
+  }
+  p.lay();
   if (dx) {
-    Epi e{};
-    e.C = dx; e.ldc = K;
-    bool done = false;
-    if constexpr (f32) done = p.template plain<true, false>(gp, ldg, w, d->ldw, M, K, N, e);
-    if (!done) {
-      const Mat A = f32 ? p.planes(gp, ldg, M, N, true) : p.half(gp, ldg, M, as_is ? N : Np);
-      const Mat B = f32 ? p.planes(w, d->ldw, N, K, false) : p.half(w, d->ldw, N, K);
-      p.template product<H, S, true, false>(A, B, M, K, N, e);
-    }
+    if constexpr (f32)
+      if (cx.tiles) p.template plain<true, false>(gp, ldg, w, d->ldw, M, K, N, ex, cx);
+    if (!cx.tiles) p.template product<H, S, true, false>(A, B, M, K, N, ex);
   }
   if (dw) {
-    Epi e{};
-    e.C = dw; e.ldc = K;
-    bool done = false;
-    if constexpr (f32) done = p.template plain<false, false>(gp, ldg, x, d->ldx, N, K, M, e);
-    if (!done) {
-      const Mat A = f32 ? p.planes(gp, ldg, M, N, false) : p.half(gp, ldg, M, as_is ? N : Np);
-      const Mat B = f32 ? p.planes(x, d->ldx, M, K, false) : p.half(x, d->ldx, M, K);
-      p.template product<H, S, false, false>(A, B, N, K, M, e);
-    }
+    if constexpr (f32)
+      if (cw.tiles) p.template plain<false, false>(gp, ldg, x, d->ldx, N, K, M, ew, cw);
+    if (!cw.tiles) p.template product<H, S, false, false>(Aw, Bw, N, K, M, ew);
   }
   return p.rc;
 }
