@@ -1042,8 +1042,8 @@ inline Shape shape_of(int M, int N, int steps, double products) {   // products:
 
 // The same for fp32 operands as they lie, 64 x 64 tiles and 32 k a step: four workgroups a CU take 2.6 us a step, 0.5 more for
 // each operand read across its rows and 1.4 for rows off 16 bytes, two and one a CU 0.55 and 0.4 of it. Measured on
-// 17 sizes in each direction, laid-out planes against this: 1365 x 83 x 76: 17, 22 and 28 us against 9, 9 and 10;
-// 1000^3: 36, 40 and 44 against 35, 38 and 39; 2048 x 1024 x 1024: 43, 47 and 55 against 47, 59 and 65.
+// 17 sizes in each direction, laid-out planes against this: 1365 x 83 x 76: 14, 23 and 21 us against 9, 9 and 10;
+// 1000^3: 29, 40 and 35 against 35, 38 and 39; 2048 x 1024 x 1024: 36, 46 and 45 against 47, 59 and 65.
 inline Shape plain_shape_of(int M, int N, int steps, double each) {
   Shape best{};
   double least = 1e300;
@@ -1161,10 +1161,10 @@ struct Pass {
     const bool avec = lda % 4 == 0 && ((uintptr_t)A & 15) == 0, bvec = ldb % 4 == 0 && ((uintptr_t)B & 15) == 0;
     auto slow = [](bool kc, bool vec) { return kc ? (vec ? 0 : 1.4) : 0.5; };
     const Shape c = plain_shape_of(M, N, (K + kPlainK - 1) / kPlainK, 2.6 + slow(AKC, avec) + slow(BKC, bvec));
-    // planes: a launch and one pass over an operand by rows, three and two by columns
-    auto laid = [](bool kc, double n) { return kc ? 5 + n * 8 / 4.5e6 : 14 + n * 12 / 4.5e6; };
-    const double planes = shape_of(M, N, (2 * ((K + 31) / 32 * 32) + kBK - 1) / kBK, 1.5).us +
-                          laid(AKC, (double)M * K) + laid(BKC, (double)N * K);
+    // planes: a launch and one pass over an operand by rows, three and two by columns, two of a kind in the same launches
+    auto laid = [](bool kc, double n) { return kc ? 4 + n * 8 / 4.5e6 : 9 + n * 12 / 4.5e6; };
+    const double planes = shape_of(M, N, (2 * ((K + 31) / 32 * 32) + kBK - 1) / kBK, 1.5).us + laid(AKC, (double)M * K) +
+                          laid(BKC, (double)N * K) - (AKC != BKC ? 0 : AKC ? 2 : 6);
     return c.us > planes || c.tiles > 0xffffff ? Shape{} : c;
   }
   template <bool AKC, bool BKC>
