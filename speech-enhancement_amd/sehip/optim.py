@@ -242,15 +242,24 @@ def _multi(params, columns, types, bits, step, lr, betas, eps, weight_decay, see
     sizes = list(map(T.numel, params))
     blocks = [-(-k // SCALE_BLOCK) for k in sizes] if bits == 8 else None
     arr = np.zeros(n, dtype=_TENSOR)
+    written = []
     for name, ts, ty in zip(_TENSOR.names, (params, *columns), (dt, *types)):
         want = blocks if name.endswith("scale") else sizes
         if (list(map(T.numel, ts)) != want or set(map(_dtype_of, ts)) != {ty} or set(map(T.get_device, ts)) != {index}
                 or not all(map(T.is_contiguous, ts))):
             raise RuntimeError(f"sehip adamw: {name}: not all contiguous {ty} tensors of the parameters' sizes on {dev}")
         arr[name] = at = list(map(T.data_ptr, ts))
-        if name != "grad" and len(set(at)) < n and len({a for a, k in zip(at, sizes) if k}) < sum(map(bool, sizes)):
-            raise RuntimeError(f"sehip adamw: the same {name} twice in the list")
+        if name == "grad":
+            grads = at
+        else:
+            written += at
+            if len(set(at)) < n and len({a for a, k in zip(at, sizes) if k}) < sum(map(bool, sizes)):
+                raise RuntimeError(f"sehip adamw: the same {name} twice in the list")
     arr["numel"] = sizes
+    if len(set(written)) < len(written) or not set(grads).isdisjoint(written):   # or some without elements
+        full = [a for a, k in zip(written, sizes * (len(written) // n)) if k]
+        if len(set(full)) < len(full) or not {a for a, k in zip(grads, sizes) if k}.isdisjoint(full):
+            raise RuntimeError("sehip adamw: one tensor in two of the lists")
     if torch.cuda.is_current_stream_capturing():
         raise RuntimeError("sehip adamw: a captured graph would repeat this step's count and bias corrections")
     N.launch(index, "se_adamw_multi", N.lib().se_adamw_multi, arr.ctypes.data, n, N.DTYPES[dt], bits, float(lr), float(betas[0]),

@@ -427,3 +427,35 @@ def test_codes_of_the_exact_states(gpu_device):
         assert (k != kg).sum() <= 1
         assert at.mean() > 0.5
         assert np.array_equal(got[at], want[at]), (got[at] != want[at]).sum()
+
+
+@pytest.mark.parametrize("bits", (8, 32))
+def test_one_tensor_in_two_lists(gpu_device, bits):
+    """Refused before anything is written: two moments, a parameter and its gradient or moment in the same memory. Tensors of no
+    elements may share an address, and two parameters a gradient."""
+    def lists():
+        f = lambda n, t: torch.ones(n, device=gpu_device, dtype=torch.uint8 if bits == 8 else torch.float32).view(  # noqa: E731
+            t if bits == 8 else torch.float32)
+        ps, gs = ([torch.ones(n, device=gpu_device) for n in (128, 0, 128)] for _ in range(2))
+        cols = [[f(n, t) for n in sizes] for t, sizes in (
+            ((torch.float8_e4m3fn, (128, 0, 128)), (torch.float8_e8m0fnu, (1, 0, 1))) * 2 if bits == 8
+            else ((None, (128, 0, 128)),) * 2)]
+        return [ps, gs, *cols]
+
+    step = optim.adamw8_ if bits == 8 else optim.adamw32_
+    step(*lists(), step=1)
+    a = lists()
+    a[1][2] = a[1][0]
+    step(*a, step=1)
+    root = 4 if bits == 8 else 3
+    for i, j in ((2, root), (0, 1), *(((3, 5),) if bits == 8 else ((0, 2), (1, 3)))):
+        for k in (0, 2):
+            a = lists()
+            a[j][k] = a[i][0]
+            with pytest.raises(RuntimeError, match="two of the lists"):
+                step(*a, step=1)
+            assert all(bool((t == 1).all()) for t in a[0])
+    a = lists()
+    flat = torch.ones(128, device=gpu_device)     # an empty slice begins where its neighbour does
+    a[0][1], a[0][2] = flat[:0], flat
+    step(*a, step=1)
