@@ -392,3 +392,31 @@ def test_fp32_as_it_lies_off_16_bytes(gpu_device):
             dy = torch.randn(90, 67, device=gpu_device)
             y, grads = _run(x, lin, "gelu", None, dy)
             _check(x, lin.weight, lin.bias, None, "gelu", dy, y, grads)
+
+
+def test_fp32_halves_in_a_graph(gpu_device):
+    """The large form's launches captured and replayed, with eager calls between: every replay gives the eager bits."""
+    x, lin, res, dy = _make(gpu_device, torch.float32, *FORMS[1], seed=14)
+    x.requires_grad_(True)
+
+    def step():
+        y = linear.linear_act(x, lin, ACTS["gelu"], res)
+        return (y, *torch.autograd.grad(y, (x, lin.weight, lin.bias), dy))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = step()
+    for k in range(4):
+        with torch.no_grad():
+            x.copy_(torch.randn(x.shape, device=gpu_device) * 2.0 ** (8 * k - 16))
+            dy.copy_(torch.randn(dy.shape, device=gpu_device) * 2.0 ** (-6 * k))
+        g.replay()
+        eager = step()
+        torch.cuda.synchronize()
+        assert all(torch.equal(p, q) for p, q in zip(out, eager)), k
