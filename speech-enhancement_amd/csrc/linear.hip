@@ -744,18 +744,29 @@ __global__ void __launch_bounds__(1024) linear_few_kernel(const S* __restrict__ 
 }
 
 // ------------------------------------------------------------------ operands laid out
-// [R][C] at ld -> rows of Cp = C rounded up to 8, zeros behind C (a matrix whose rows do not start on 16 bytes)
-__global__ void __launch_bounds__(256) linear_pack_kernel(const u16* __restrict__ x, long long ld, int R, int C, int Cp,
-                                                          u16* __restrict__ out) {
-  const int per = Cp / 8;
-  const long long total = (long long)R * per;
+// [R][C] at ld -> rows of Cp = C rounded up to 8, zeros behind C (a matrix whose rows do not start on 16 bytes). A launch
+// takes the operands of a pass side by side (blockIdx.z), since alone the small ones take what a launch takes.
+constexpr int kMostJobs = 3;
+struct PackJob {
+  const u16* x;
+  u16* out;
+  long long ld;
+  int R, C, Cp;
+};
+struct PackJobs {
+  PackJob j[kMostJobs];
+};
+__global__ void __launch_bounds__(256) linear_pack_kernel(const PackJobs jobs) {
+  const PackJob& t = jobs.j[blockIdx.z];
+  const int per = t.Cp / 8, C = t.C;
+  const long long total = (long long)t.R * per;
   for (long long i = blockIdx.x * 256LL + threadIdx.x; i < total; i += gridDim.x * 256LL) {
     const int r = (int)(i / per), c = (int)(i - (long long)r * per) * 8;
-    const u16* p = x + r * ld + c;
+    const u16* p = t.x + r * t.ld + c;
     s16x8 v;
 #pragma unroll
     for (int j = 0; j < 8; ++j) v[j] = c + j < C ? (short)p[j] : (short)0;
-    *reinterpret_cast<s16x8*>(out + (long long)r * Cp + c) = v;
+    *reinterpret_cast<s16x8*>(t.out + (long long)r * t.Cp + c) = v;
   }
 }
 
@@ -793,8 +804,7 @@ __device__ __forceinline__ void split_two(float a, float b, int ea, int eb, unsi
   hi = __builtin_bit_cast(unsigned, (f16x2){h0, h1});
   lo = __builtin_bit_cast(unsigned, (f16x2){l0, l1});
 }
-// An operand to be laid out. A launch takes the operands of a pass side by side (blockIdx.z), since alone the small ones
-// take what a launch takes.
+// an operand to be laid out, of a launch's several (blockIdx.z)
 struct SplitJob {
   const float* x;   // [R][C] at ld
   long long ld;
@@ -805,7 +815,6 @@ struct SplitJob {
   int rows, parts;
   bool two, known;  // two: pairs are aligned; known: `part` is there
 };
-constexpr int kMostJobs = 3;
 struct SplitJobs {
   SplitJob j[kMostJobs];
 };
@@ -1074,7 +1083,9 @@ struct Pass {
     if (rc == SE_OK && hipGetLastError() != hipSuccess) rc = SE_E_LAUNCH;
   }
 
-  // 16-bit [R][C] at ld, as it is or packed
+  // 16-bit [R][C] at ld, as it is or packed (by lay())
+  PackJobs packs{};
+  int n_packs = 0;
   Mat half(const void* x, long long ld, int R, int C) {
     Mat m{};
     if (ld % 8 == 0 && C % 8 == 0 && ((uintptr_t)x & 15) == 0) {
@@ -1085,11 +1096,7 @@ struct Pass {
     }
     const int Cp = up8(C);
     u16* out = ws.take<u16>((long long)R * Cp);
-    if (run) {
-      hipLaunchKernelGGL(linear_pack_kernel, dim3(blocks_for((long long)R * Cp / 8)), dim3(256), 0, st,
-                         static_cast<const u16*>(x), ld, R, C, Cp, out);
-      launched();
-    }
+    packs.j[n_packs++] = PackJob{static_cast<const u16*>(x), out, ld, R, C, Cp};
     m.p = out;
     m.ld = Cp;
     m.bytes = (long long)R * Cp * 2;
@@ -1125,6 +1132,11 @@ struct Pass {
   }
   void lay() {
     if (!run || rc != SE_OK) return;
+    if (n_packs) {
+      unsigned blocks = 0;
+      for (int i = 0; i < n_packs; ++i) blocks = std::max(blocks, blocks_for((long long)packs.j[i].R * packs.j[i].Cp / 8));
+      hipLaunchKernelGGL(linear_pack_kernel, dim3(blocks, 1, n_packs), dim3(256), 0, st, packs);
+    }
     if (n_rows) {
       long long most = 0;
       for (int i = 0; i < n_rows; ++i) most = std::max(most, (by_rows.j[i].R + 3LL) / 4);
@@ -1144,7 +1156,7 @@ struct Pass {
       hipLaunchKernelGGL(linear_col_exp_kernel, dim3((C + 63) / 64, 1, n_cols), dim3(1024), 0, st, by_cols);
       hipLaunchKernelGGL(linear_split_cols_kernel, dim3(blocks, 1, n_cols), dim3(256), 0, st, by_cols);
     }
-    n_rows = n_cols = 0;
+    n_packs = n_rows = n_cols = 0;
     launched();
   }
 
@@ -1332,7 +1344,7 @@ int backward(const se_linear_desc* d, const void* dy, const void* x, const void*
     B = f32 ? p.planes(w, d->ldw, N, K, false) : p.half(w, d->ldw, N, K);
   }
   if (dw && !cw.tiles) {
-    Aw = f32 ? p.planes(gp, ldg, M, N, false, top, tops ? parts : 0) : p.half(gp, ldg, M, as_is ? N : Np);
+    Aw = f32 ? p.planes(gp, ldg, M, N, false, top, tops ? parts : 0) : dx ? A : p.half(gp, ldg, M, as_is ? N : Np);
     Bw = f32 ? p.planes(x, d->ldx, M, K, false) : p.half(x, d->ldx, M, K);
   }
   p.lay();
