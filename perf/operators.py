@@ -26,19 +26,13 @@ SIZE = {"f32": 4, "bf16": 2, "f16": 2}
 ACTS = ("none", "relu", "gelu", "gelu_tanh", "silu")
 
 
-_PACKAGE = []
-
-
 def _sehip():
-    """The package's folder is put on the path as bench.py does it; a program imports it once."""
-    if _PACKAGE:
-        return _PACKAGE
+    """The package's folder is put on the path as bench.py does it."""
     at = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "speech-enhancement_amd")
     if at not in sys.path:
         sys.path.insert(0, at)
     from sehip import linear, norm, optim
-    _PACKAGE[:] = linear, norm, optim
-    return _PACKAGE
+    return linear, norm, optim
 
 
 # ---------------------------------------------------------------------------------------------- the cases
