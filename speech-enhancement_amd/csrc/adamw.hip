@@ -6,16 +6,19 @@
 // 32: m and v in fp32. 8: m and q = sqrt(v) as e4m3 values times one power of two for each 128 consecutive
 // elements of a tensor (codes [numel], exponents k + 127 [ceil(numel / 128)]). q rather than v: half the binades, so
 // e4m3's 18 below the block's largest cover gradients down to 2^-18 of it. k is the smallest with amax <= 448 2^k.
-// Rounding is stochastic: the magnitude in grid steps plus u = (h + 1/2) / 65536, rounded down, h the low (m) or high (q)
-// half of a hash of (seed, step, tensor, element). To the nearest, a state would stand still: a step moves v by
-// 1 - b2 = 0.001 of it, half a grid step is 2^-4. The hash is a counter's, so the replicas of a data-parallel run, which
-// share seed and gradients, keep the same states. A positive q is stored as at least the smallest value: as 0 it
-// would leave m' / eps. The parameter moves by m' and v' before they are rounded.
+// m', v' ((1 - b2) g before times g) and q are fp32 values, each operation rounded once in the order it is written in, the same at 8
+// and at 32 bits, and a code is the exact rounding of the fp32 value: a program that takes the step in elementary fp32
+// operations holds the same codes, however often it is taken (a code that differs moves the next step's parameter by up
+// to a tenth of lr). Rounding is stochastic: the magnitude in grid steps plus u = (h + 1/2) / 65536, rounded down, h the
+// low (m) or high (q) half of a hash of (seed, step, tensor, element). To the nearest, a state would stand still: a step
+// moves v by 1 - b2 = 0.001 of it, half a grid step is 2^-4. The hash is a counter's, so the replicas of a data-parallel
+// run, which share seed and gradients, keep the same states. A positive q is stored as at least the smallest value: as 0
+// it would leave m' / eps. The parameter moves by m' and v' before they are rounded to codes.
 //
 // Bound by memory: at 8 bits an element of an fp32 parameter reads and writes 16.06 bytes. The table of tensors goes in
 // the kernel's arguments (no copy, no device table to keep alive, 48 tensors a launch); a workgroup takes one
 // chunk of 2048 consecutive elements of one tensor, eight a thread, so 16 lanes share a block's exponent. 336 M fp32
-// parameters with 8-bit states: 1.05 ms, 5.1 TB/s (a large copy: 5.0); 67 M bf16 ones with 32-bit states: 297 us, 5.0.
+// parameters with 8-bit states: 1.01 ms, 5.3 TB/s (a large copy: 5.0); 67 M bf16 ones with 32-bit states: 297 us, 5.0.
 #include "common.hpp"
 
 #include <cmath>
@@ -44,7 +47,6 @@ struct Table {
 };
 struct Hyper {
   float decay, w1, b2, omb2, inv_bc2_sqrt, eps, neg_step;
-  float w1_lo, b2_lo, omb2_lo;   // what the 32 bits of each leave over
 };
 static_assert(sizeof(Table) + sizeof(Hyper) <= 4096, "kernel arguments");
 
@@ -109,39 +111,11 @@ __device__ __forceinline__ void load_codes(const unsigned char* p, bool vec, int
   }
 }
 
-// A code is a step function of the state and of h, and the errors of 32-bit arithmetic turn about one in a million, that lies
-// next to its border. A code within kNear of one is taken again from the state as hi + lo, lo what hi's rounding
-// left over: the products' and sums' errors by fma and by the two-sum of Knuth, q's from s - q^2 = 2 q lo.
-// 336 M parameters in 1.05 ms against 1.02 without; every state in twice the bits took 1.26, the flagged waves'
-// states all eight again 1.15 (95 registers, five waves a SIMD).
-constexpr float kNear = 0x1p-17f;   // the errors: a few 2^-24 of a value of up to 16
-__device__ __forceinline__ void two_sum(float a, float b, float& s, float& e) {
+// m' and v' from m and v, no two operations joined into one rounding
+__device__ __forceinline__ void moments(const Hyper& h, float g, float& m, float& v) {
 #pragma clang fp contract(off)
-  s = a + b;
-  const float t = s - a;
-  e = (a - (s - t)) + (b - t);
-}
-__device__ __forceinline__ void step_m(const Hyper& h, float g, float& m, float& lo) {
-#pragma clang fp contract(off)
-  float d, ed, s, es;
-  two_sum(g, -m, d, ed);
-  const float p = h.w1 * d;
-  two_sum(m, p, s, es);
-  lo = es + (__builtin_fmaf(h.w1, d, -p) + __builtin_fmaf(h.w1, ed, h.w1_lo * d));
-  m = s;
-}
-// v: q^2 on entry (q of 4 bits: exact), q on return
-__device__ __forceinline__ void step_q(const Hyper& h, float g, float& v, float& lo) {
-#pragma clang fp contract(off)
-  const float a = h.b2 * v, gg = g * g, c = h.omb2 * gg;
-  float s, es;
-  two_sum(a, c, s, es);
-  const float ea = __builtin_fmaf(h.b2, v, -a) + h.b2_lo * v;
-  const float ec = __builtin_fmaf(h.omb2, gg, -c);
-  const float eg = __builtin_fmaf(h.omb2, __builtin_fmaf(g, g, -gg), h.omb2_lo * gg);
-  const float q = sqrtf(s);
-  lo = q > 0.f ? (__builtin_fmaf(-q, q, s) + (es + (ea + (ec + eg)))) * 0.5f * __builtin_amdgcn_rcpf(q) : 0.f;
-  v = q;
+  m = m + h.w1 * (g - m);
+  v = h.b2 * v + h.omb2 * g * g;
 }
 
 // k + 127 of the block that this thread's sixteen lanes hold: amax over their finite values
@@ -159,26 +133,17 @@ __device__ __forceinline__ unsigned block_exp(const float (&v)[8]) {
   return (unsigned)max(k, 1);
 }
 
-// e4m3 code of x 2^-k, rounded stochastically by the 16 bits h; NaN for what is not finite. EXACT: of x + lo
-template <bool EXACT>
-__device__ __forceinline__ unsigned code_of(float x, float lo, float inv, unsigned h, bool floor1, bool& near) {
+// e4m3 code of x 2^-k, rounded stochastically by the 16 bits h; NaN for what is not finite. z, its fraction and 1 - u are
+// fp32 numbers without an error, so that the comparison is the exact one (z + u would be rounded, at times up to the border).
+__device__ __forceinline__ unsigned code_of(float x, float inv, unsigned h, bool floor1) {
 #pragma clang fp contract(off)
   const float a = fabsf(x);
   const float y = a * inv;
   const int e = max((int)(__builtin_bit_cast(unsigned, y) >> 23) - 127, -6);
-  const float z = __builtin_ldexpf(y, 3 - e), u = ((float)h + 0.5f) * 0x1p-16f;   // z: 8 .. 16, or less below 2^-6
-  float f;
-  if constexpr (EXACT) {
-    float t, et;
-    two_sum(z, u, t, et);
-    f = floorf(t);
-    if (f == t && et + __builtin_ldexpf((x < 0.f ? -lo : lo) * inv, 3 - e) < 0.f) f -= 1.f;   // a little below f
-  } else {
-    const float t = z + u;
-    f = floorf(t);
-    near = fabsf(t - rintf(t)) < kNear;
-  }
-  unsigned c = (unsigned)(((e + 7) << 3) + (int)f - 8);
+  const float z = __builtin_ldexpf(y, 3 - e);   // 8 .. 16, or less below 2^-6
+  const float f = floorf(z);
+  const bool up = z - f >= ((float)(0xffffu - h) + 0.5f) * 0x1p-16f;
+  unsigned c = (unsigned)(((e + 7) << 3) + (int)f - 8 + up);
   if (floor1 && a > 0.f) c = max(c, 1u);
   if (!(a < INFINITY)) c = 0x7fu;
   return c | ((__builtin_bit_cast(unsigned, x) >> 24) & 0x80u);
@@ -227,8 +192,7 @@ __global__ void __launch_bounds__(kThr) adamw_multi_kernel(const Table tab, cons
   }
 #pragma unroll
   for (int j = 0; j < 8; ++j) {
-    m[j] = m[j] + h.w1 * (g[j] - m[j]);
-    v[j] = h.b2 * v[j] + h.omb2 * (g[j] * g[j]);
+    moments(h, g[j], m[j], v[j]);
     const float q = sqrtf(v[j]);
     p[j] = p[j] * h.decay + h.neg_step * m[j] / (q * h.inv_bc2_sqrt + h.eps);
     if constexpr (Q8) v[j] = q;
@@ -240,38 +204,12 @@ __global__ void __launch_bounds__(kThr) adamw_multi_kernel(const Table tab, cons
     const float mi = __builtin_bit_cast(float, (254u - nmk) << 23), vi = __builtin_bit_cast(float, (254u - nvk) << 23);
     unsigned char* cm = static_cast<unsigned char*>(t.m) + i;
     unsigned char* cv = static_cast<unsigned char*>(t.v) + i;
-    unsigned wm[2] = {0u, 0u}, wv[2] = {0u, 0u}, again = 0;
+    unsigned wm[2] = {0u, 0u}, wv[2] = {0u, 0u};
 #pragma unroll
     for (int j = 0; j < 8; ++j) {   // i is a multiple of 8: the upper half is the same for all eight
       const unsigned r = mix(base + j * 0x9E3779B1u);
-      bool nm, nv;
-      wm[j >> 2] |= code_of<false>(m[j], 0.f, mi, r & 0xffffu, false, nm) << (8 * (j & 3));
-      wv[j >> 2] |= code_of<false>(v[j], 0.f, vi, r >> 16, true, nv) << (8 * (j & 3));
-      again |= (j < left && (nm || nv)) ? 1u << j : 0u;
-    }
-    while (again) {   // one element in thirty thousand: its codes are still in memory
-      const int j = __builtin_ctz(again);
-      again &= again - 1;
-      const unsigned r = mix(base + j * 0x9E3779B1u);
-      const float gj = (float)static_cast<const T*>(t.g)[i + j];
-      float mj = __builtin_amdgcn_cvt_f32_fp8((int)cm[j], 0) * __builtin_bit_cast(float, mk << 23);
-      float vj = __builtin_amdgcn_cvt_f32_fp8((int)cv[j], 0) * __builtin_bit_cast(float, vk << 23);
-      float ml, vl;
-      bool n;
-      vj *= vj;
-      step_m(h, gj, mj, ml);
-      step_q(h, gj, vj, vl);
-      const int at = 8 * (j & 3);
-      const unsigned keep = ~(0xffu << at);
-      const unsigned a = code_of<true>(mj, ml, mi, r & 0xffffu, false, n) << at;
-      const unsigned b = code_of<true>(vj, vl, vi, r >> 16, true, n) << at;
-      if (j < 4) {
-        wm[0] = (wm[0] & keep) | a;
-        wv[0] = (wv[0] & keep) | b;
-      } else {
-        wm[1] = (wm[1] & keep) | a;
-        wv[1] = (wv[1] & keep) | b;
-      }
+      wm[j >> 2] |= code_of(m[j], mi, r & 0xffffu, false) << (8 * (j & 3));
+      wv[j >> 2] |= code_of(v[j], vi, r >> 16, true) << (8 * (j & 3));
     }
     store_codes(cm, vec, left, wm[0], wm[1]);
     store_codes(cv, vec, left, wv[0], wv[1]);
@@ -313,9 +251,6 @@ extern "C" int se_adamw_multi(const se_adamw_tensor* tensors, int n, int dtype, 
   h.w1 = (float)(1.0 - beta1);
   h.b2 = (float)beta2;
   h.omb2 = (float)(1.0 - beta2);
-  h.w1_lo = (float)((1.0 - beta1) - h.w1);
-  h.b2_lo = (float)(beta2 - h.b2);
-  h.omb2_lo = (float)((1.0 - beta2) - h.omb2);
   h.inv_bc2_sqrt = (float)(1.0 / std::sqrt(1.0 - std::pow(beta2, (double)step)));
   h.eps = (float)eps;
   h.neg_step = (float)(-(lr / (1.0 - std::pow(beta1, (double)step))));
