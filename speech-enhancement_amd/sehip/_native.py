@@ -59,11 +59,19 @@ class GemmDesc(ctypes.Structure):
         (n, c_int) for n in ("kmask_period", "kmask_phase", "splits", "dtype", "bias_rows")]
 
 
+INT_MAX = 0x7fffffff
+
+
 class LinearDesc(ctypes.Structure):
     """Mirror of se_linear_desc (include/sehip.h, ABI 12)."""
 
     _fields_ = [(n, c_int) for n in ("M", "N", "K", "act", "dtype")] + [
         (n, ctypes.c_longlong) for n in ("ldx", "ldw", "ldr")]
+
+    def __init__(self, M, N, K, *rest):
+        if M > INT_MAX or N > INT_MAX or K > INT_MAX:   # ctypes would keep their low 32 bits
+            raise RuntimeError(f"sehip linear: {M} x {K} -> {N}: sizes behind 32-bit indexes")
+        super().__init__(M, N, K, *rest)
 
 
 _P = c_void_p

@@ -275,6 +275,8 @@ def linear_act(x: torch.Tensor, module: nn.Linear, act: nn.Module | None = None,
     n, k = w.shape
     if n == 0 or k == 0 or x.dim() == 0 or x.shape[-1] != k:
         raise RuntimeError(f"sehip linear_act: input {tuple(x.shape)}, weight {tuple(w.shape)}")
+    if x.numel() // k > N.INT_MAX:   # before anything of that size is made
+        raise RuntimeError(f"sehip linear_act: input {tuple(x.shape)}: rows behind 32-bit indexes")
     if residual is not None and residual.shape != x.shape[:-1] + (n,):
         raise RuntimeError(f"sehip linear_act: residual {tuple(residual.shape)}, output {tuple(x.shape[:-1]) + (n,)} (it is "
                            "not broadcast)")

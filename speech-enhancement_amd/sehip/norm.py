@@ -176,14 +176,11 @@ def layer_norm(norm: nn.LayerNorm, x: torch.Tensor) -> torch.Tensor:
                            "in its type or both in fp32)")
     if not ((w is None or w.is_contiguous()) and (b is None or b.is_contiguous())):
         raise RuntimeError("sehip layer_norm: weight and bias must be contiguous")
+    C = shape[0] if k == 1 else math.prod(shape)
+    if not 0 < C <= N.INT_MAX:
+        raise RuntimeError("sehip layer_norm: normalised over " + ("no elements" if C == 0 else f"{C} elements: behind 32-bit indexes"))
     if k == 1:
-        C = shape[0]
-        if C == 0:
-            raise RuntimeError("sehip layer_norm: normalised over no elements")
         return _layer_norm(x, w, b, C, norm.eps)
-    C = math.prod(shape)
-    if C == 0:
-        raise RuntimeError("sehip layer_norm: normalised over no elements")
     # the normalised axes as one (views of w and b, so that their gradients come back in their own shapes)
     return _layer_norm(x.flatten(x.dim() - k), w if w is None else w.view(C), b if b is None else b.view(C), C,
                        norm.eps).view(x.shape)
