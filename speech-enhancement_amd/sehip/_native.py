@@ -13,6 +13,7 @@ import os
 import re
 
 import torch  # noqa: F401  (must precede the CDLL load, see module doc)
+import torch.autograd.forward_ad as _fwad
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
 # SEHIP_LIB may point at another in-tree build of the same library (A/B
@@ -272,6 +273,12 @@ def _raw_stream(index: int) -> int:
 # the same two answers without the objects around them, where this torch has them (a launch's host time)
 _get_device = getattr(torch._C, "_cuda_getDevice", _get_device)
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", _raw_stream)
+
+
+def followed() -> bool:
+    """Whether a dual level or a trace is open: an operator goes through its autograd.Function then, gradients wanted or not,
+    so that a tangent is refused instead of dropped and the trace holds the call."""
+    return _fwad._current_level >= 0 or torch.jit.is_tracing()
 
 
 def ptr(t) -> int | None:

@@ -262,7 +262,7 @@ def linear_act(x: torch.Tensor, module: nn.Linear, act: nn.Module | None = None,
     fp32 (large products on each operand split into two scaled fp16 planes, fp32-class), bf16 and fp16 (exact
     products, fp32 sums, one rounding of the result). act: nn.Identity / None, nn.ReLU, nn.GELU (both forms) or nn.SiLU. For the backward the
     pre-activation is kept in the storage type. In fp32 an infinity or NaN in x or W makes what it reaches infinite or
-    NaN, not always the one of the two that fp32 products would give. A second derivative is refused."""
+    NaN, not always the one of the two that fp32 products would give. A second derivative and one in forward mode are refused."""
     code = _act_code(act)
     w, b = module.weight, module.bias
     dev, dt = x.get_device(), x.dtype
@@ -283,7 +283,7 @@ def linear_act(x: torch.Tensor, module: nn.Linear, act: nn.Module | None = None,
     if b is not None and not b.is_contiguous():
         raise RuntimeError("sehip linear_act: the bias must be contiguous")
     LINEAR_CALLS[0] += 1
-    if torch.is_grad_enabled() and (x.requires_grad or w.requires_grad or (b is not None and b.requires_grad)
-                                    or (residual is not None and residual.requires_grad)):
+    if (torch.is_grad_enabled() and (x.requires_grad or w.requires_grad or (b is not None and b.requires_grad)
+                                     or (residual is not None and residual.requires_grad))) or N.followed():
         return _LinearAct.apply(x, w, b, residual, code)
     return _act_forward(x, w, b, residual, code, False)[0]

@@ -160,7 +160,7 @@ class _LayerNorm(torch.autograd.Function):
 def layer_norm(norm: nn.LayerNorm, x: torch.Tensor) -> torch.Tensor:
     """norm(x) on the HIP kernels: x [..., *norm.normalized_shape] on the GPU in fp32, bf16 or fp16; norm's weight
     and bias (each may be absent) both in x's type or both in fp32. The result is contiguous, in x's type. A second
-    derivative is refused."""
+    derivative and one in forward mode are refused."""
     shape, w, b = norm.normalized_shape, norm.weight, norm.bias
     k = len(shape)
     if x.shape[-k:] != shape:
@@ -187,7 +187,7 @@ def layer_norm(norm: nn.LayerNorm, x: torch.Tensor) -> torch.Tensor:
 
 
 def _layer_norm(x, w, b, C, eps):
-    if torch.is_grad_enabled() and (x.requires_grad or (w is not None and w.requires_grad)
-                                    or (b is not None and b.requires_grad)):
+    if (torch.is_grad_enabled() and (x.requires_grad or (w is not None and w.requires_grad)
+                                     or (b is not None and b.requires_grad))) or N.followed():
         return _LayerNorm.apply(x, w, b, C, eps)
     return _ln_forward(x, C, w, b, eps, False)[0]
