@@ -805,9 +805,10 @@ int se_layer_norm_bwd(const void* dy, long long dy_stride, const void* x, long l
  * fp32 accumulation, y rounded once.
  * Backward: g = dy act'(z) (dy's rows ldr apart), dx = g W, dw = g^T x,
  * db = sum_m g; what is not NULL is written, z is needed where act is not
- * SE_LINACT_NONE. N, K and the strides up to 2^21, M up to 2^28, each matrix up
- * to 2^37 elements; more is SE_E_UNSUPPORTED. The workspace sizes depend on the
- * pointers' alignment; the forward of up to SE_LINEAR_FEW_ROWS rows takes none.
+ * SE_LINACT_NONE. N and K up to 2^21, M up to 2^28, each matrix up to 2^37
+ * elements; more is SE_E_UNSUPPORTED. Rows may lie any distance apart. The
+ * workspace sizes depend on the pointers' alignment and on the distances; the
+ * forward of up to SE_LINEAR_FEW_ROWS rows takes none.
  * ------------------------------------------------------------------------ */
 enum {
   SE_LINACT_NONE = 0,

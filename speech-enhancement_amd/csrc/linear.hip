@@ -44,6 +44,7 @@ typedef unsigned short u16;
 
 constexpr int kBK = 64;
 constexpr int kTop = 14;
+constexpr int kMostLd = 1 << 21;   // elements between rows that the tiled product reads: its byte offsets in a tile are 32-bit
 
 struct Epi {
   void* C;              // [M][N]
@@ -1083,12 +1084,12 @@ struct Pass {
     if (rc == SE_OK && hipGetLastError() != hipSuccess) rc = SE_E_LAUNCH;
   }
 
-  // 16-bit [R][C] at ld, as it is or packed (by lay())
+  // 16-bit [R][C] at ld, as it is or packed (by lay()): off 16 bytes, or rows further apart than a tile's offsets reach
   PackJobs packs{};
   int n_packs = 0;
   Mat half(const void* x, long long ld, int R, int C) {
     Mat m{};
-    if (ld % 8 == 0 && C % 8 == 0 && ((uintptr_t)x & 15) == 0) {
+    if (ld % 8 == 0 && C % 8 == 0 && ((uintptr_t)x & 15) == 0 && ld <= kMostLd) {
       m.p = static_cast<const u16*>(x);
       m.ld = ld;
       m.bytes = ((long long)(R - 1) * ld + C) * 2;
@@ -1206,7 +1207,7 @@ struct Pass {
     a.e = e;
     a.e.ea = A.ex; a.e.eb = B.ex;
     if (__is_same(S, float)) a.K = 2 * ((K + 31) / 32 * 32);   // 32 k of hi and of lo to a tile
-    if (A.ld > (1 << 22) || B.ld > (1 << 22)) { rc = SE_E_UNSUPPORTED; return; }
+    if (A.ld > 2 * kMostLd || B.ld > 2 * kMostLd) { rc = SE_E_UNSUPPORTED; return; }   // hi and lo side by side
     a.steps = (a.K + kBK - 1) / kBK;
     const Shape c = shape_of(M, N, a.steps, sizeof(S) == 4 ? 1.5 : 1);
     a.per = c.per;
@@ -1367,8 +1368,7 @@ int check(const se_linear_desc* d) {
   if (d->act < SE_LINACT_NONE || d->act > SE_LINACT_SILU) return SE_E_ARG;
   if (d->ldw < d->K || d->ldx < 0 || (d->M > 1 && d->ldx < d->K) || d->ldr < 0 || (d->M > 1 && d->ldr && d->ldr < d->N))
     return SE_E_ARG;
-  if (d->N > (1 << 21) || d->K > (1 << 21) || d->ldw > (1LL << 21) || d->ldx > (1LL << 21) || d->ldr > (1LL << 21))
-    return SE_E_UNSUPPORTED;   // a tile's byte offsets are 32-bit
+  if (d->N > kMostLd || d->K > kMostLd) return SE_E_UNSUPPORTED;
   // indexes of rows are 32-bit, of fp32's hi and lo rows too; a launch has less than 2^32 threads
   const long long most = 1LL << 37, M = d->M, N = d->N, K = d->K;
   if (M > (1 << 28) || M * N > most || M * K > most || N * K > most) return SE_E_UNSUPPORTED;
