@@ -91,7 +91,7 @@ class AdamW(torch.optim.Optimizer):
     per-parameter steps) is updated by its own launch with its own bias
     corrections, as torch tracks the step per parameter.
 
-    state_bits None: the moments in the parameters' type (torch's state layout). 32: state[p] =
+    state_bits (a group may have its own, and its own seed) None: the moments in the parameters' type (torch's state layout). 32: state[p] =
     {'step', 'exp_avg', 'exp_avg_sq'} with fp32 moments. 8: {'step', 'exp_avg', 'exp_avg_scale',
     'exp_avg_root', 'exp_avg_root_scale'}, e4m3 values of m and sqrt(v) and their e8m0 powers of two,
     rounded stochastically from `seed`: the replicas of a data-parallel run, given one seed and the same
@@ -105,10 +105,19 @@ class AdamW(torch.optim.Optimizer):
         defaults = dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, amsgrad=False, maximize=False,
                         foreach=None, capturable=False, differentiable=False, fused=None)
         if state_bits is not None:
-            if state_bits not in (8, 32):
-                raise ValueError(f"sehip AdamW: state_bits {state_bits!r} (None, 8 or 32)")
-            defaults.update(state_bits=int(state_bits), seed=int(seed))
+            defaults.update(state_bits=state_bits, seed=int(seed))
+        self._seed = int(seed)
         super().__init__(params, defaults)
+
+    def add_param_group(self, param_group):
+        """As torch's; a group may have its own state_bits and seed."""
+        bits = param_group.get("state_bits", self.defaults.get("state_bits")) if isinstance(param_group, dict) else None
+        if bits is not None:
+            if bits not in (8, 32):
+                raise ValueError(f"sehip AdamW: state_bits {bits!r} (None, 8 or 32)")
+            param_group["state_bits"] = int(bits)
+            param_group["seed"] = int(param_group.get("seed", getattr(self, "_seed", 0)))
+        super().add_param_group(param_group)
 
     def load_state_dict(self, state_dict):
         """As torch's, but the moments of state_bits 8 / 32 keep their own type (torch casts a state to its

@@ -13,3 +13,18 @@ def test_sizes_that_a_c_int_does_not_hold(sizes):
     with pytest.raises(RuntimeError, match="32-bit"):
         N.LinearDesc(*sizes, 0, 1, 8, 8, 4)
     assert N.LinearDesc((1 << 31) - 1, 4, 8, 0, 1, 8, 8, 4).M == (1 << 31) - 1
+
+
+def test_a_group_with_its_own_state_bits():
+    p = lambda: nn.Parameter(torch.zeros(3))  # noqa: E731
+    o = optim.AdamW([{"params": [p()], "state_bits": 8}, {"params": [p()], "state_bits": 32, "seed": 9}, {"params": [p()]}], seed=4)
+    assert [(g.get("state_bits"), g.get("seed")) for g in o.param_groups] == [(8, 4), (32, 9), (None, None)]
+    o.add_param_group({"params": [p()], "state_bits": 8})
+    assert o.param_groups[-1]["seed"] == 4 and "state_bits" not in o.param_groups[2]
+    o = optim.AdamW([{"params": [p()]}, {"params": [p()], "state_bits": None}], state_bits=8, seed=2)
+    assert [(g["state_bits"], g["seed"]) for g in o.param_groups] == [(8, 2), (None, 2)]
+    for bad in (16, "8", 0, -8):
+        with pytest.raises(ValueError, match="state_bits"):
+            optim.AdamW([{"params": [p()], "state_bits": bad}])
+        with pytest.raises(ValueError, match="state_bits"):
+            o.add_param_group({"params": [p()], "state_bits": bad})

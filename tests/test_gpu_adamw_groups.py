@@ -1,0 +1,35 @@
+"""AdamW(state_bits=8): groups with settings of their own, and the random bits of a group's tensors."""
+import pytest
+import torch
+import torch.nn as nn
+
+from sehip import optim
+
+pytestmark = pytest.mark.gpu
+HP = dict(lr=1e-3, betas=(0.9, 0.999), eps=1e-8, weight_decay=1e-2)
+
+
+def _codes(o, p):
+    return [t.view(torch.uint8).clone() for k, t in o.state[p].items() if k in ("exp_avg", "exp_avg_root")]
+
+
+def _step(ps, **kw):
+    o = optim.AdamW(ps, **kw, **HP)
+    for p in (p for g in o.param_groups for p in g["params"]):
+        p.grad = torch.full_like(p, 0.3)
+    o.step()
+    return o
+
+
+def test_a_group_with_its_own_state_bits(gpu_device):
+    f = lambda: nn.Parameter(torch.ones(300, device=gpu_device))  # noqa: E731
+    a, b, c = f(), f(), f()
+    o = _step([{"params": [a], "state_bits": 8}, {"params": [b], "state_bits": 32}, {"params": [c]}])
+    assert set(o.state[a]) == {"step", "exp_avg", "exp_avg_scale", "exp_avg_root", "exp_avg_root_scale"}
+    assert o.state[b]["exp_avg"].dtype == torch.float32 and set(o.state[c]) == {"step", "exp_avg", "exp_avg_sq"}
+    assert torch.equal(a, b) and (a - c).abs().max() <= 1e-6
+    d, e = f(), f()
+    o = _step([{"params": [d], "seed": 5}, {"params": [e]}], state_bits=8, seed=5)
+    p = _step([f()], state_bits=8, seed=5)
+    assert all(torch.equal(x, y) for x, y in zip(_codes(o, d), _codes(p, p.param_groups[0]["params"][0])))
+    assert not torch.equal(_codes(o, d)[0], _codes(o, e)[0])
