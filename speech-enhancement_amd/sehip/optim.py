@@ -121,8 +121,8 @@ class AdamW(torch.optim.Optimizer):
 
     def load_state_dict(self, state_dict):
         """As torch's, but the moments of state_bits 8 / 32 keep their own type (torch casts a state to its
-        parameter's). A state without the keys or types of this optimizer's state_bits is refused, except that
-        state_bits 32 takes moments of any floating type."""
+        parameter's). A state without the keys or types of this optimizer's state_bits is refused before anything
+        is replaced; None and 32 take moments of any floating type of 16 bits or more."""
         given = state_dict["state"]
         ids = [i for g in state_dict["param_groups"] for i in g["params"]]
         mine = [(p, g.get("state_bits")) for g in self.param_groups for p in g["params"]]
@@ -130,13 +130,20 @@ class AdamW(torch.optim.Optimizer):
             return super().load_state_dict(state_dict)
         keep = []
         for i, (p, bits) in zip(ids, mine):
-            if bits is None or i not in given:
+            if i not in given:
+                continue
+            if bits is None:   # torch would take 8-bit codes, without their scales, for numbers
+                for key in ("exp_avg", "exp_avg_sq") if given[i] else ():
+                    t = given[i].get(key)
+                    if t is None or not t.is_floating_point() or t.element_size() == 1:
+                        raise ValueError(f"sehip AdamW: the loaded state has no {key} for state_bits=None")
                 continue
             keep.append((p, "step", torch.as_tensor(given[i]["step"]).clone()))
             want = _state_like(p, bits)
             for key, like in want.items():
                 t = given[i].get(key)
-                if t is None or t.shape != like.shape or (t.dtype != like.dtype if bits == 8 else not t.is_floating_point()):
+                if t is None or t.shape != like.shape or (
+                        t.dtype != like.dtype if bits == 8 else not t.is_floating_point() or t.element_size() == 1):
                     raise ValueError(f"sehip AdamW: the loaded state has no {key} for state_bits={bits}")
                 keep.append((p, key, t.to(device=p.device, dtype=like.dtype, copy=True)))
         own = [{k: g[k] for k in ("state_bits", "seed") if k in g} for g in self.param_groups]

@@ -28,3 +28,24 @@ def test_a_group_with_its_own_state_bits():
             optim.AdamW([{"params": [p()], "state_bits": bad}])
         with pytest.raises(ValueError, match="state_bits"):
             o.add_param_group({"params": [p()], "state_bits": bad})
+
+
+@pytest.mark.parametrize("to", (None, 32))
+def test_a_state_of_8_bits_is_not_taken_for_numbers(to):
+    """torch casts what it loads to the parameter's type: codes without their scales. Refused, and nothing is replaced."""
+    make = lambda bits: optim.AdamW([nn.Parameter(torch.zeros(7, 40)), nn.Parameter(torch.zeros(3))], lr=0.5, state_bits=bits)  # noqa: E731
+    a, b = make(8), make(to)
+    p = a.param_groups[0]["params"][0]
+    a.state[p] = {"step": torch.tensor(4.0), **optim._state_like(p, 8, torch.zeros)}
+    a.param_groups[0]["lr"] = 0.25
+    q = b.param_groups[0]["params"][0]
+    b.state[q] = {"step": torch.tensor(2.0), "exp_avg": torch.ones(7, 40), "exp_avg_sq": torch.ones(7, 40)}
+    with pytest.raises(ValueError, match="exp_avg"):
+        b.load_state_dict(a.state_dict())
+    assert b.param_groups[0]["lr"] == 0.5 and float(b.state[q]["step"]) == 2 and set(b.state[q]) == {"step", "exp_avg", "exp_avg_sq"}
+    t = torch.optim.AdamW([nn.Parameter(torch.zeros(7, 40)), nn.Parameter(torch.zeros(3))], lr=0.125)
+    r = t.param_groups[0]["params"][0]
+    r.grad = torch.ones_like(r)
+    t.step()
+    b.load_state_dict(t.state_dict())
+    assert b.param_groups[0]["lr"] == 0.125 and torch.equal(b.state[q]["exp_avg"], t.state[r]["exp_avg"])
