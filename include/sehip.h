@@ -839,8 +839,8 @@ int se_linear_bwd(const se_linear_desc* d, const void* dy, const void* x, const 
  * and a scale byte (k + 127 for 2^k) for each SE_ADAMW_BLOCK consecutive
  * elements, [ceil(numel / SE_ADAMW_BLOCK)]; k is the smallest with
  * amax <= 448 2^k (at least -126). Rounding is stochastic with 16 bits of a hash
- * of (seed, step, index of the tensor in the table, element); a positive sqrt(v) is stored as
- * the smallest code at least; what is not finite is stored as NaN and leaves its
+ * of (all 64 bits of seed, step, index of the tensor in the table, element); a
+ * positive sqrt(v) is stored as the smallest code at least; what is not finite is stored as NaN and leaves its
  * block's scale alone. What is rounded are the fp32 m + (1 - b1) (g - m) and
  * sqrt(b2 v + (1 - b2) g g), each operation rounded once in that order (what bits 32
  * holds), exactly. The parameter moves by m and v before they are rounded to codes

@@ -254,7 +254,7 @@ extern "C" int se_adamw_multi(const se_adamw_tensor* tensors, int n, int dtype, 
   h.inv_bc2_sqrt = (float)(1.0 / std::sqrt(1.0 - std::pow(beta2, (double)step)));
   h.eps = (float)eps;
   h.neg_step = (float)(-(lr / (1.0 - std::pow(beta1, (double)step))));
-  const unsigned k0 = mix(mix((unsigned)seed) + (unsigned)step);
+  const unsigned k0 = mix(mix((unsigned)seed + mix((unsigned)(seed >> 32))) + (unsigned)step);   // mix(0) is 0
   hipStream_t st = se::as_stream(stream);
   Table tab;
   tab.n = 0;

@@ -33,3 +33,11 @@ def test_a_group_with_its_own_state_bits(gpu_device):
     p = _step([f()], state_bits=8, seed=5)
     assert all(torch.equal(x, y) for x, y in zip(_codes(o, d), _codes(p, p.param_groups[0]["params"][0])))
     assert not torch.equal(_codes(o, d)[0], _codes(o, e)[0])
+
+
+def test_all_bits_of_the_seed_count(gpu_device):
+    out = [_codes(o, o.param_groups[0]["params"][0]) for o in
+           (_step([nn.Parameter(torch.ones(3000, device=gpu_device))], state_bits=8, seed=s) for s in (7, 7 + (1 << 32), 7 + (1 << 63)))]
+    for i in range(3):
+        for j in range(i):
+            assert not torch.equal(out[i][0], out[j][0]) and not torch.equal(out[i][1], out[j][1])
