@@ -205,11 +205,11 @@ class AdamW(torch.optim.Optimizer):
                 st.update(_state_like(p, bits, torch.zeros))
             calls.setdefault((int(st["step"].item()) + 1, p.dtype, p.device), []).append(p)
         kw = dict(lr=group["lr"], betas=group["betas"], eps=group["eps"], weight_decay=group["weight_decay"])
-        for (step, _, _), ps in sorted(calls.items(), key=lambda c: c[0][0]):
+        for call, ((step, _, _), ps) in enumerate(sorted(calls.items(), key=lambda c: c[0][0])):
             sts = [self.state[p] for p in ps]
             states = [[st[k] for st in sts] for k in _STATE_KEYS[bits]]
-            if bits == 8:   # a group's own stream of random bits
-                adamw8_(ps, [p.grad for p in ps], *states, step=step, seed=group["seed"] + 0x10001 * at, **kw)
+            if bits == 8:   # random bits of the group's own, and of each call's (which counts its tensors from 0)
+                adamw8_(ps, [p.grad for p in ps], *states, step=step, seed=group["seed"] + 0x10001 * at + (call << 32), **kw)
             else:
                 adamw32_(ps, [p.grad for p in ps], *states, step=step, **kw)
             for st in sts:   # counted once the launch has gone through

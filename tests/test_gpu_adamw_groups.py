@@ -35,6 +35,24 @@ def test_a_group_with_its_own_state_bits(gpu_device):
     assert not torch.equal(_codes(o, d)[0], _codes(o, e)[0])
 
 
+def test_types_side_by_side_have_their_own_random_bits(gpu_device):
+    """One group of fp32, bf16 and fp16 tensors of the same values: m' = 0.03 in each, its rounding from bits of its own."""
+    n = 1 << 14
+    ps = [nn.Parameter(torch.full((n,), 0.5, device=gpu_device, dtype=t)) for t in (torch.float32, torch.bfloat16, torch.float16)]
+    o = optim.AdamW(ps, state_bits=8, seed=5, **HP)
+    for p in ps:
+        p.grad = torch.full_like(p, 0.296875)    # a number of every type
+    o.step()
+    every = [_codes(o, p) for p in ps]
+    for i in range(3):
+        for j in range(i):
+            for a, b in zip(every[i], every[j]):
+                # two values an element: independent bits agree at half to all but a few (share s of the upper one: s^2 + (1-s)^2)
+                s = [(t == t.max()).double().mean().item() for t in (a, b)]
+                agree, want = (a == b).double().mean().item(), s[0] * s[1] + (1 - s[0]) * (1 - s[1])
+                assert abs(agree - want) < 6 * 0.5 / n ** 0.5, (i, j, agree, want)
+
+
 def test_all_bits_of_the_seed_count(gpu_device):
     out = [_codes(o, o.param_groups[0]["params"][0]) for o in
            (_step([nn.Parameter(torch.ones(3000, device=gpu_device))], state_bits=8, seed=s) for s in (7, 7 + (1 << 32), 7 + (1 << 63)))]
