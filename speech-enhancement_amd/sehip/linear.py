@@ -182,16 +182,17 @@ _FEW_ROWS = 64   # SE_LINEAR_FEW_ROWS (include/sehip.h): up to so many rows the 
 ACT_NONE, ACT_RELU, ACT_GELU, ACT_GELU_TANH, ACT_SILU = range(5)   # SE_LINACT_* (include/sehip.h)
 
 
+_ACTS = ((nn.Identity, ACT_NONE), (nn.ReLU, ACT_RELU), (nn.GELU, ACT_GELU), (nn.SiLU, ACT_SILU))
+
+
 def _act_code(act) -> int:
-    """SE_LINACT_* of an activation module (an inplace flag makes no difference: z is the kernel's own)."""
-    if act is None or isinstance(act, nn.Identity):
+    """SE_LINACT_* of an activation module (an inplace flag makes no difference: z is the kernel's own). A subclass counts as
+    its base where it has no forward of its own."""
+    if act is None:
         return ACT_NONE
-    if isinstance(act, nn.GELU):
-        return ACT_GELU_TANH if act.approximate == "tanh" else ACT_GELU
-    if isinstance(act, nn.SiLU):
-        return ACT_SILU
-    if type(act) is nn.ReLU:
-        return ACT_RELU
+    for cls, code in _ACTS:
+        if isinstance(act, cls) and type(act).forward is cls.forward:
+            return ACT_GELU_TANH if code == ACT_GELU and act.approximate == "tanh" else code
     raise NotImplementedError(f"sehip linear_act: activation {type(act).__name__} (Identity, ReLU, GELU, SiLU)")
 
 

@@ -49,3 +49,19 @@ def test_a_state_of_8_bits_is_not_taken_for_numbers(to):
     t.step()
     b.load_state_dict(t.state_dict())
     assert b.param_groups[0]["lr"] == 0.125 and torch.equal(b.state[q]["exp_avg"], t.state[r]["exp_avg"])
+
+
+@pytest.mark.parametrize("base", (nn.Identity, nn.ReLU, nn.GELU, nn.SiLU))
+def test_an_activation_with_a_forward_of_its_own(base):
+    """Refused; a subclass that only adds something else is its base."""
+    class Scaled(base):
+        def forward(self, x):
+            return 2 * super().forward(x)
+
+    class Named(base):
+        name = "named"
+
+    with pytest.raises(NotImplementedError, match="Scaled"):
+        linear.linear_act(torch.zeros(3, 8), nn.Linear(8, 4), Scaled())
+    assert linear._act_code(Named()) == linear._act_code(base())
+    assert linear._act_code(nn.GELU("tanh")) == linear.ACT_GELU_TANH != linear._act_code(nn.GELU())
