@@ -61,6 +61,7 @@ class GemmDesc(ctypes.Structure):
 
 
 INT_MAX = 0x7fffffff
+_struct_init = ctypes.Structure.__init__
 
 
 class LinearDesc(ctypes.Structure):
@@ -72,7 +73,7 @@ class LinearDesc(ctypes.Structure):
     def __init__(self, M, N, K, *rest):
         if M > INT_MAX or N > INT_MAX or K > INT_MAX:   # ctypes would keep their low 32 bits
             raise RuntimeError(f"sehip linear: {M} x {K} -> {N}: sizes behind 32-bit indexes")
-        super().__init__(M, N, K, *rest)
+        _struct_init(self, M, N, K, *rest)
 
 
 _P = c_void_p
@@ -273,12 +274,13 @@ def _raw_stream(index: int) -> int:
 # the same two answers without the objects around them, where this torch has them (a launch's host time)
 _get_device = getattr(torch._C, "_cuda_getDevice", _get_device)
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", _raw_stream)
+_is_tracing = getattr(torch._C, "_is_tracing", torch.jit.is_tracing)
 
 
 def followed() -> bool:
     """Whether a dual level or a trace is open: an operator goes through its autograd.Function then, gradients wanted or not,
     so that a tangent is refused instead of dropped and the trace holds the call."""
-    return _fwad._current_level >= 0 or torch.jit.is_tracing()
+    return _fwad._current_level >= 0 or _is_tracing()
 
 
 def ptr(t) -> int | None:
