@@ -28,7 +28,8 @@
 extern "C" {
 #endif
 
-#define SEHIP_ABI_VERSION 12  /* 12: se_layer_norm_fwd / _bwd, se_linear_fwd / _bwd (bias, activation and residual
+#define SEHIP_ABI_VERSION 13  /* 13: se_linear_tile;
+                                 12: se_layer_norm_fwd / _bwd, se_linear_fwd / _bwd (bias, activation and residual
                                  in the epilogue), se_adamw_multi (states in 8 or 32 bits);
                                  11: se_cbn_bwd_ccbam (the CCBAM gate's input gradient formed inside the
                                  encoder CBN backward);
@@ -830,6 +831,10 @@ size_t se_linear_bwd_workspace_size(const se_linear_desc* d, const void* dy, con
                                     int want_dx, int want_dw, int want_db);
 int se_linear_bwd(const se_linear_desc* d, const void* dy, const void* x, const void* w, const void* z, void* dx,
                   void* dw, void* db, void* ws, size_t ws_bytes, void* stream);
+/* What multiplies `product` (0: y, 1: dx, 2: dw) for operands on 16 bytes: the side of the tiled product's tile (256 or
+ * 128), 64 for fp32 as it lies, 0 for the few rows' kernel; *splits (or NULL): the parts of the reduced length. Negative:
+ * an error. (ABI 13) */
+int se_linear_tile(const se_linear_desc* d, int product, int* splits);
 
 /* ------------------------------------------------------------------------
  * One AdamW step (decoupled decay, amsgrad off) over n tensors (ABI 12), their

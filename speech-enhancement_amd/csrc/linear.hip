@@ -186,8 +186,8 @@ struct Cols {
   }
 };
 
-// those columns of row m, out of the sums; res: the residual's values. Every row is aligned for V.
-template <typename S, int V, bool RES>
+// those columns of row m, out of the sums; res: the residual's values, or zeros. Every row is aligned for V.
+template <typename S, int V>
 __device__ __forceinline__ void epilogue(const Epi& e, const Cols<S, V>& cols, long long m, int n, float (&v)[V],
                                          const float (&res)[V], int ea) {
   if constexpr (sizeof(S) == 4)   // fp32: the planes' powers of two (0 where there are none)
@@ -197,9 +197,8 @@ __device__ __forceinline__ void epilogue(const Epi& e, const Cols<S, V>& cols, l
   for (int j = 0; j < V; ++j) v[j] += cols.bias[j];
   if (e.z) store_pack<S, V>(static_cast<S*>(e.z) + m * e.ldz + n, v);
   act_of<sizeof(S) == 2, V>(e.act, v);
-  if constexpr (RES)
 #pragma unroll
-    for (int j = 0; j < V; ++j) v[j] += res[j];
+  for (int j = 0; j < V; ++j) v[j] += res[j];
   store_pack<S, V>(static_cast<S*>(e.C) + m * e.ldc + n, v);
 }
 
@@ -580,7 +579,7 @@ __global__ void __launch_bounds__(256) linear_join_kernel(const GemmArgs a) {
 #pragma unroll
     for (int j = 0; j < V; ++j) res[j] = 0.f;
     if (a.e.res) load_pack<S, V>(static_cast<const S*>(a.e.res) + m * a.e.ldr + n, res);
-    epilogue<S, V, true>(a.e, cols, m, n, v, res, a.e.ea ? a.e.ea[m] : 0);
+    epilogue<S, V>(a.e, cols, m, n, v, res, a.e.ea ? a.e.ea[m] : 0);
   }
 }
 
@@ -659,7 +658,7 @@ __global__ void __launch_bounds__(256) linear_plain_kernel(const GemmArgs a, boo
     } else {
       float v[1] = {acc[i]}, res[1] = {0.f};
       if (a.e.res) res[0] = static_cast<const float*>(a.e.res)[m * a.e.ldr + n];
-      epilogue<float, 1, true>(a.e, cols, m, n, v, res, 0);
+      epilogue<float, 1>(a.e, cols, m, n, v, res, 0);
     }
   }
 }
@@ -742,7 +741,7 @@ __global__ void __launch_bounds__(1024) linear_few_kernel(const S* __restrict__ 
     Cols<S, 1> cols;
     cols.load(e, n);
     if (e.res) res[0] = (float)static_cast<const S*>(e.res)[m * e.ldr + n];
-    epilogue<S, 1, true>(e, cols, m, n, v, res, 0);
+    epilogue<S, 1>(e, cols, m, n, v, res, 0);
   }
 }
 
@@ -1082,6 +1081,7 @@ struct Pass {
   bool run;
   hipStream_t st;
   int rc = SE_OK;
+  int tile = 0, splits = 1;   // of the last product; tile 0: none was chosen
   void launched() {
     if (rc == SE_OK && hipGetLastError() != hipSuccess) rc = SE_E_LAUNCH;
   }
@@ -1193,7 +1193,8 @@ struct Pass {
     a.steps = (K + kPlainK - 1) / kPlainK;
     const bool avec = lda % 4 == 0 && ((uintptr_t)A & 15) == 0, bvec = ldb % 4 == 0 && ((uintptr_t)B & 15) == 0;
     a.per = c.per;
-    a.splits = (a.steps + a.per - 1) / a.per;
+    a.splits = splits = (a.steps + a.per - 1) / a.per;
+    tile = c.tile;
     if (a.splits > 1) a.slab = ws.take<float>((long long)a.splits * M * N);
     if (!run || rc != SE_OK) return;
     hipLaunchKernelGGL((linear_plain_kernel<AKC, BKC>), dim3((unsigned)c.tiles, a.splits), dim3(256), 0, st, a, avec, bvec);
@@ -1213,7 +1214,8 @@ struct Pass {
     a.steps = (a.K + kBK - 1) / kBK;
     const Shape c = shape_of(M, N, a.steps, sizeof(S) == 4 ? 1.5 : 1);
     a.per = c.per;
-    a.splits = (a.steps + a.per - 1) / a.per;
+    a.splits = splits = (a.steps + a.per - 1) / a.per;
+    tile = c.tile;
     if (a.splits > 1) a.slab = ws.take<float>((long long)a.splits * M * N);
     if (!run || rc != SE_OK) return;
     const bool res = e.res && a.splits == 1;
@@ -1420,6 +1422,19 @@ extern "C" size_t se_linear_bwd_workspace_size(const se_linear_desc* d, const vo
   char some;   // only asked whether it is there
   backward_any(d, dy, x, w, nullptr, want_dx ? &some : nullptr, want_dw ? &some : nullptr, want_db ? &some : nullptr, p);
   return p.ws.at;
+}
+
+extern "C" int se_linear_tile(const se_linear_desc* d, int product, int* splits) {
+  const int rc = check(d);
+  if (rc != SE_OK) return rc;
+  if (product < 0 || product > 2) return SE_E_ARG;
+  Pass p{Carve{nullptr}, false, nullptr};
+  char* some = reinterpret_cast<char*>(256);   // on 16 bytes, never read
+  if (product == 0) forward_any(d, some, some, nullptr, nullptr, nullptr, nullptr, p);
+  else backward_any(d, some, some, some, nullptr, product == 1 ? some : nullptr, product == 2 ? some : nullptr, nullptr, p);
+  if (p.rc != SE_OK) return p.rc;
+  if (splits) *splits = p.splits;
+  return p.tile;
 }
 
 extern "C" int se_linear_bwd(const se_linear_desc* d, const void* dy, const void* x, const void* w, const void* z, void* dx,

@@ -77,7 +77,7 @@ class LinearDesc(ctypes.Structure):
 
 
 _P = c_void_p
-ABI_VERSION = 12   # SEHIP_ABI_VERSION (include/sehip.h)
+ABI_VERSION = 13   # SEHIP_ABI_VERSION (include/sehip.h)
 CBN_SAVE_FLOATS = 20   # SE_CBN_SAVE_FLOATS (include/sehip.h)
 _PP = ctypes.POINTER(c_void_p)   # host array of device pointers
 _SIGNATURES = {
@@ -198,6 +198,7 @@ _SIGNATURES = {
     "se_linear_fwd": (c_int, [_P] * 8 + [c_size_t, _P]),
     "se_linear_bwd_workspace_size": (c_size_t, [_P] * 4 + [c_int] * 3),
     "se_linear_bwd": (c_int, [_P] * 9 + [c_size_t, _P]),
+    "se_linear_tile": (c_int, [_P, c_int, _P]),
     "se_adamw_multi": (c_int, [_P, c_int, c_int, c_int] + [ctypes.c_double] * 5 + [ctypes.c_longlong,
                                                                                   ctypes.c_ulonglong, _P]),
     "se_complex_join": (c_int, [_P, c_int, c_int, c_int, _P, c_int, c_int, c_int, _P, c_int, c_int, _P]),

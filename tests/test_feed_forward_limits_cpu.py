@@ -1,4 +1,6 @@
 """The feed-forward operators' calls at the edges of what they take: refused or answered on the host, without a GPU."""
+import ctypes
+
 import pytest
 import torch
 import torch.nn as nn
@@ -65,3 +67,20 @@ def test_an_activation_with_a_forward_of_its_own(base):
         linear.linear_act(torch.zeros(3, 8), nn.Linear(8, 4), Scaled())
     assert linear._act_code(Named()) == linear._act_code(base())
     assert linear._act_code(nn.GELU("tanh")) == linear.ACT_GELU_TANH != linear._act_code(nn.GELU())
+
+
+def test_linear_tile():
+    """What multiplies a product is known on the host."""
+    def tile(dt, m, k, n, product, act=0):
+        splits = ctypes.c_int(-1)
+        t = N.lib().se_linear_tile(ctypes.byref(N.LinearDesc(m, n, k, act, dt, k, k, n)), product, ctypes.byref(splits))
+        return t, splits.value
+
+    F32, BF16 = 0, 1
+    for p in range(3):
+        assert tile(BF16, 16384, 4096, 8192, p, 3) == (256, 1)
+        assert tile(F32, 100, 64, 72, p)[0] == 64
+    assert tile(BF16, 16, 4096, 1024, 0) == (0, 1) and tile(BF16, 16, 4096, 1024, 1)[0] == 128   # few rows: forward alone
+    assert tile(BF16, 1000, 64, 72, 0) == (128, 1) and tile(BF16, 20000, 64, 48, 2)[1] > 1
+    assert tile(BF16, 100, 64, 72, 3)[0] == tile(BF16, 0, 64, 72, 0)[0] == -1
+    assert N.lib().se_linear_tile(ctypes.byref(N.LinearDesc(100, 64, 72, 0, 1, 72, 72, 64)), 0, None) == 128
