@@ -27,7 +27,9 @@ _LL5 = ctypes.c_longlong * 5
 
 
 def copy_into(src: torch.Tensor, dst: torch.Tensor) -> torch.Tensor:
-    """dst[...] = src[...] (same shape, any strides, storage types converted) in one launch."""
+    """dst[...] = src[...] (same shape, any strides, storage types converted) in one launch (a lazily negated src, as the
+    imaginary part of a conjugate is, is resolved first: the kernels read memory)."""
+    src = src.resolve_neg()
     if tuple(src.shape) != tuple(dst.shape):
         raise ValueError(f"sehip copy: shapes {tuple(src.shape)} and {tuple(dst.shape)} differ")
     N.require_device(src, dtype=src.dtype)
@@ -54,6 +56,7 @@ def copy_into(src: torch.Tensor, dst: torch.Tensor) -> torch.Tensor:
 def as_rows(t: torch.Tensor, C: int, dtype=None):
     """(t2, ld): t as rows of C contiguous elements ld apart, in `dtype`; copied (se_copy_strided) only where its
     strides or its type are others. For kernels that read [rows, C] matrices; not differentiable."""
+    t = t.resolve_neg()
     if dtype is None or t.dtype == dtype:
         if t.is_contiguous():
             return t, C
@@ -81,7 +84,7 @@ class _Contig(torch.autograd.Function):
 def contiguous(x: torch.Tensor, dtype=None) -> torch.Tensor:
     """x.contiguous().to(dtype) as one HIP pass (x itself when nothing changes)."""
     dtype = dtype or x.dtype
-    if x.is_contiguous() and x.dtype == dtype:
+    if x.is_contiguous() and x.dtype == dtype and not x.is_neg():
         return x
     return _Contig.apply(x, dtype)
 

@@ -229,7 +229,7 @@ def _act_backward(ctx, gy):
     dw = new((n, k)) if need[1] else None
     db = new(n) if need[2] else None
     if m and (need[0] or need[1] or need[2]):
-        g2, ldg = (gy, n) if gy.is_contiguous() and gy.dtype == x.dtype else glue.as_rows(gy, n, x.dtype)
+        g2, ldg = (gy, n) if gy.is_contiguous() and gy.dtype == x.dtype and not gy.is_neg() else glue.as_rows(gy, n, x.dtype)
         w2, ldw = (w, k) if w.is_contiguous() else glue.as_rows(w, k)
         lib = N.lib()
         p = ctypes.byref(N.LinearDesc(m, n, k, act, N.DTYPES[x.dtype], ldx, ldw, ldg))
@@ -283,6 +283,8 @@ def linear_act(x: torch.Tensor, module: nn.Linear, act: nn.Module | None = None,
                            "not broadcast)")
     if b is not None and not b.is_contiguous():
         raise RuntimeError("sehip linear_act: the bias must be contiguous")
+    if x.is_neg() or w.is_neg() or (b is not None and b.is_neg()) or (residual is not None and residual.is_neg()):
+        x, w, b, residual = (t if t is None else t.resolve_neg() for t in (x, w, b, residual))
     LINEAR_CALLS[0] += 1
     if (torch.is_grad_enabled() and (x.requires_grad or w.requires_grad or (b is not None and b.requires_grad)
                                      or (residual is not None and residual.requires_grad))) or N.followed():

@@ -131,7 +131,7 @@ def _ln_backward(ctx, gy):
     dw = new(C, dtype=wdt) if need[1] else None
     db = new(C, dtype=wdt) if need[2] else None
     if rows:
-        g2, ldg = (gy, C) if gy.is_contiguous() and gy.dtype == x.dtype else glue.as_rows(gy, C, x.dtype)
+        g2, ldg = (gy, C) if gy.is_contiguous() and gy.dtype == x.dtype and not gy.is_neg() else glue.as_rows(gy, C, x.dtype)
         lib = N.lib()
         size = lib.se_layer_norm_workspace_size(rows, C) if need[1] or need[2] else 0
         ws = x.new_empty(size, dtype=torch.uint8) if size else None
@@ -176,6 +176,8 @@ def layer_norm(norm: nn.LayerNorm, x: torch.Tensor) -> torch.Tensor:
                            "in its type or both in fp32)")
     if not ((w is None or w.is_contiguous()) and (b is None or b.is_contiguous())):
         raise RuntimeError("sehip layer_norm: weight and bias must be contiguous")
+    if x.is_neg() or (w is not None and w.is_neg()) or (b is not None and b.is_neg()):
+        x, w, b = (t if t is None else t.resolve_neg() for t in (x, w, b))
     C = shape[0] if k == 1 else math.prod(shape)
     if not 0 < C <= N.INT_MAX:
         raise RuntimeError("sehip layer_norm: normalised over " + ("no elements" if C == 0 else f"{C} elements: behind 32-bit indexes"))

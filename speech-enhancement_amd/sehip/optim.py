@@ -177,7 +177,7 @@ class AdamW(torch.optim.Optimizer):
                     st["exp_avg_sq"] = torch.zeros_like(p, memory_format=torch.preserve_format)
                 st["step"] += 1
                 s = int(st["step"].item())   # a CPU tensor, as torch's non-capturable AdamW
-                by_step.setdefault(s, []).append((p, p.grad, st["exp_avg"], st["exp_avg_sq"]))
+                by_step.setdefault(s, []).append((p, p.grad.resolve_neg(), st["exp_avg"], st["exp_avg_sq"]))
             b1, b2 = group["betas"]
             for step_val, rows in sorted(by_step.items()):
                 by_dtype: dict = {}
@@ -249,6 +249,8 @@ def _multi(params, columns, types, bits, step, lr, betas, eps, weight_decay, see
         raise ValueError(f"sehip adamw: step {step} (counted from 1)")
     if not (0.0 <= betas[0] < 1.0 and 0.0 <= betas[1] < 1.0):
         raise ValueError(f"sehip adamw: betas {betas}")
+    if any(map(torch.Tensor.is_neg, columns[0])):   # one element that is an imaginary part: negated lazily
+        columns = ([g.resolve_neg() for g in columns[0]], *columns[1:])
     p0 = params[0]
     dev, dt = p0.device, p0.dtype
     if dev.type != "cuda" or dt not in N.DTYPES:
