@@ -282,8 +282,7 @@ def _multi(params, columns, types, bits, step, lr, betas, eps, weight_decay, see
         raise RuntimeError("sehip adamw: a captured graph would repeat this step's count and bias corrections")
     N.launch(index, "se_adamw_multi", N.lib().se_adamw_multi, arr.ctypes.data, n, N.DTYPES[dt], bits, float(lr), float(betas[0]),
              float(betas[1]), float(eps), float(weight_decay), int(step), int(seed) & 0xFFFFFFFFFFFFFFFF)
-    written = [*params, *columns[1], *columns[2]]
-    torch.autograd.graph.increment_version(written)
+    torch.autograd.graph.increment_version([t for ts in (params, *columns[1:]) for t in ts])
 
 
 @torch.no_grad()

@@ -59,3 +59,14 @@ def test_all_bits_of_the_seed_count(gpu_device):
     for i in range(3):
         for j in range(i):
             assert not torch.equal(out[i][0], out[j][0]) and not torch.equal(out[i][1], out[j][1])
+
+
+@pytest.mark.parametrize("bits", (8, 32))
+def test_everything_written_counts_as_changed(gpu_device, bits):
+    """Autograd finds a saved tensor changed by its version: parameters, moments and scales each get a new one, gradients none."""
+    f = lambda n, t: torch.ones(n, device=gpu_device, dtype=torch.uint8 if t.itemsize == 1 else t).view(t)  # noqa: E731
+    kinds = [(5, torch.float32)] * 2 + ([(5, torch.float8_e4m3fn), (1, torch.float8_e8m0fnu)] * 2 if bits == 8 else [(5, torch.float32)] * 2)
+    lists = [[f(n, t)] for n, t in kinds]
+    before = [ts[0]._version for ts in lists]
+    (optim.adamw8_ if bits == 8 else optim.adamw32_)(*lists, step=1)
+    assert [ts[0]._version - v for ts, v in zip(lists, before)] == [1, 0] + [1] * (len(lists) - 2)
