@@ -182,7 +182,7 @@ _FEW_ROWS = 64   # SE_LINEAR_FEW_ROWS (include/sehip.h): up to so many rows the 
 ACT_NONE, ACT_RELU, ACT_GELU, ACT_GELU_TANH, ACT_SILU = range(5)   # SE_LINACT_* (include/sehip.h)
 
 
-_ACTS = ((nn.Identity, ACT_NONE), (nn.ReLU, ACT_RELU), (nn.GELU, ACT_GELU), (nn.SiLU, ACT_SILU))
+_ACTS = {nn.Identity: ACT_NONE, nn.ReLU: ACT_RELU, nn.GELU: ACT_GELU, nn.SiLU: ACT_SILU}
 
 
 def _act_code(act) -> int:
@@ -190,10 +190,12 @@ def _act_code(act) -> int:
     its base where it has no forward of its own."""
     if act is None:
         return ACT_NONE
-    for cls, code in _ACTS:
-        if isinstance(act, cls) and type(act).forward is cls.forward:
-            return ACT_GELU_TANH if code == ACT_GELU and act.approximate == "tanh" else code
-    raise NotImplementedError(f"sehip linear_act: activation {type(act).__name__} (Identity, ReLU, GELU, SiLU)")
+    code = _ACTS.get(type(act))
+    if code is None:
+        code = next((c for cls, c in _ACTS.items() if isinstance(act, cls) and type(act).forward is cls.forward), None)
+    if code is None:
+        raise NotImplementedError(f"sehip linear_act: activation {type(act).__name__} (Identity, ReLU, GELU, SiLU)")
+    return ACT_GELU_TANH if code == ACT_GELU and act.approximate == "tanh" else code
 
 
 def _act_forward(x, w, b, res, act, keep):
