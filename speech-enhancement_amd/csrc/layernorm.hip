@@ -231,7 +231,8 @@ __global__ void __launch_bounds__(NT > 256 ? NT : 256) ln_bwd_kernel(const LnArg
   }
 }
 
-// Rows wider than 1024 threads hold (16384, or 8192 of odd width): three passes over the row, which the L2 keeps
+// Rows wider than 1024 threads hold (16384): three passes over the row, which the L2 keeps, one element a load. Not
+// made fast: 2048 x 20000 fp32 forward 111 us (3.0 TB/s), 2048 x 40000 bf16 270 us (1.2 TB/s).
 template <typename T>
 __global__ void __launch_bounds__(1024) ln_fwd_wide_kernel(const LnArgs a) {
   __shared__ float red[2 * 2 * 16];
@@ -345,9 +346,15 @@ inline bool aligned(const void* p, long long stride_bytes, int n) {
   return ((uintptr_t)p % n) == 0 && stride_bytes % n == 0;
 }
 
-// Workgroups that stay, each with its columns' weights in registers: the forward at 32768 x 4096 bf16 takes 100 us (5.4 TB/s) with
-// 1536 (six a CU), 129 with 1024 and 112 to 130 with 2048 and more; read for every row, the weights made it 130. The
-// backward takes 165 us (4.9 TB/s) with 1024, 200 with 512 or 1280.
+// Workgroups that stay, each with its columns' weights in registers (read for every row they made the forward at 32768 x 4096
+// bf16 130 us). 1536 (six a CU) and 1024 were chosen at that size (256 threads a row); 768, 1024, 1536, 2048 and 3072
+// forward, 512, 768, 1024, 1536 and 2048 backward take, in us:
+//   threads  rows x columns       forward                 backward
+//   16       65536 x 64 bf16      9   8   7   8   8       17  17  19  24  27
+//   64       25792 x 514 fp32     19  19  20  20  19      42  39  37  43  43
+//   64       65536 x 200 bf16     15  14  12  14  13      26  26  27  34  37
+//   256      32768 x 4096 bf16    142 120 103 123 105     184 160 167 192 193
+//   1024     4096 x 16384 bf16    54  70  57  59  58      105 133 127 178 153   (a third forward, half backward)
 constexpr int kFwdGroups = 1536;
 constexpr int kMaxParts = 1024;
 

@@ -264,7 +264,7 @@ def linear_act(x: torch.Tensor, module: nn.Linear, act: nn.Module | None = None,
     """act(module(x)) + residual in one product: x [..., in], residual [..., out] (or None), all on one GPU in one of
     fp32 (large products on each operand split into two scaled fp16 planes, fp32-class), bf16 and fp16 (exact
     products, fp32 sums, one rounding of the result). act: nn.Identity / None, nn.ReLU, nn.GELU (both forms) or nn.SiLU. For the backward the
-    pre-activation is kept in the storage type. In fp32 an infinity or NaN in x or W makes what it reaches infinite or
+    pre-activation is kept in the storage type, and dy act' is rounded to it before the gradients' products. In fp32 an infinity or NaN in x or W makes what it reaches infinite or
     NaN, not always the one of the two that fp32 products would give. A second derivative and one in forward mode are refused."""
     code = _act_code(act)
     w, b = module.weight, module.bias
