@@ -347,14 +347,14 @@ inline bool aligned(const void* p, long long stride_bytes, int n) {
 }
 
 // Workgroups that stay, each with its columns' weights in registers (read for every row they made the forward at 32768 x 4096
-// bf16 130 us). 1536 (six a CU) and 1024 were chosen at that size (256 threads a row); 768, 1024, 1536, 2048 and 3072
-// forward, 512, 768, 1024, 1536 and 2048 backward take, in us:
-//   threads  rows x columns       forward                 backward
-//   16       65536 x 64 bf16      9   8   7   8   8       17  17  19  24  27
-//   64       25792 x 514 fp32     19  19  20  20  19      42  39  37  43  43
-//   64       65536 x 200 bf16     15  14  12  14  13      26  26  27  34  37
-//   256      32768 x 4096 bf16    142 120 103 123 105     184 160 167 192 193
-//   1024     4096 x 16384 bf16    54  70  57  59  58      105 133 127 178 153   (a third forward, half backward)
+// bf16 130 us). 1536 (six a CU) and 1024 were chosen at that size (256 threads a row); 768, 1024, 1536 and 2048 forward,
+// 512, 768, 1024 and 2048 backward take, in us:
+//   threads  rows x columns       forward             backward
+//   16       65536 x 64 bf16      9   8   7   8       17  17  19  27
+//   64       25792 x 514 fp32     19  19  20  20      42  39  37  43
+//   64       65536 x 200 bf16     15  14  12  14      26  26  27  37
+//   256      32768 x 4096 bf16    142 120 103 123     184 160 167 193
+//   1024     4096 x 16384 bf16    54  70  57  59      105 133 127 178   (a third of them forward, half backward)
 constexpr int kFwdGroups = 1536;
 constexpr int kMaxParts = 1024;
 
